@@ -48,6 +48,8 @@ typedef struct CUstream_st* llmc_stream_t; /* == cudaStream_t */
 #define LLMC_STATUS_APPEND_OVERFLOW 4
 #define LLMC_STATUS_ROPE_RANGE 8
 #define LLMC_STATUS_SEQLEN_RANGE 16
+#define LLMC_STATUS_BAD_GROUP 32
+#define LLMC_STATUS_BAD_PARENT 64
 
 /* llmc_paged_decode / llmc_rope_append_decode_strided flags */
 #define LLMC_DECODE_FORCE_GENERIC 1 /* use the SIMT kernel even where the TMA kernel applies */
@@ -253,6 +255,82 @@ LLMC_API int llmc_paged_decode_noalloc(const void* q, const void* k_pages, const
 
 /* Bytes of the built-in scratch of llmc_paged_decode_noalloc (no counterpart in the reference). */
 LLMC_API size_t llmc_paged_decode_noalloc_capacity_bytes(void);
+
+/*
+ * Paged decode attention for a batch whose sequences share prefixes (beams of a prompt,
+ * requests behind one system prompt).  No counterpart in the reference, which decodes one
+ * sequence; same result as llmc_paged_decode, but the shared tokens of a group are read
+ * once for all its sequences.  16-bit scores are not rounded to the tensor type here:
+ * scores, softmax statistics and partials are fp32, and out is rounded once.
+ *
+ *   q, out [B, Hq, d]; k_pages, v_pages, block_table, seq_lens as llmc_paged_decode: every
+ *     row of the table names all of its sequence's pages, the shared ones included.
+ *   group_starts [num_groups + 1] int32: group g holds the sequences
+ *     [group_starts[g], group_starts[g + 1]).  Groups ascend and do not overlap (otherwise
+ *     LLMC_STATUS_BAD_GROUP); a sequence in no group reads all its tokens itself.
+ *     0 <= num_groups <= B.
+ *   shared_lens [num_groups] int32: the first shared_lens[g] tokens of the group's
+ *     sequences are the same tokens.  Any length, also inside a page; 0: nothing shared.
+ *     They are read through the row of the group's first non-empty sequence, and only up
+ *     to the length of the group's shortest non-empty one.
+ *   max_group: bound on the sequences of a group, sizes the workspace; sequences of a
+ *     group beyond it read all their tokens themselves.
+ *   An empty sequence (seq_lens 0) gives zeros; its table row is not read.
+ *   workspace: llmc_shared_prefix_workspace_bytes bytes, 16-byte aligned, any content;
+ *     calls that may run at the same time need one each.
+ * All lengths are read on the device.  flags: LLMC_DECODE_FORCE_GENERIC or 0.
+ */
+LLMC_API size_t llmc_shared_prefix_workspace_bytes(int B, int Hq, int Hkv, int d, int page_size,
+                                                   int num_groups, int max_group, int dtype);
+LLMC_API int llmc_shared_prefix_decode(
+    const void* q, const void* k_pages, const void* v_pages, const int32_t* block_table,
+    const int32_t* seq_lens, const int32_t* group_starts, const int32_t* shared_lens, void* out,
+    void* workspace, size_t workspace_bytes, int32_t* status, int B, int Hq, int Hkv, int d,
+    int page_size, int max_pages_per_seq, int num_pages, int num_groups, int max_group,
+    float scale, int dtype, int flags, llmc_stream_t stream);
+
+/*
+ * Beam selection: for each of G prompts the n best continuations of its K beams,
+ *   score[k, v] = beam_scores[k] + logits[k, v] - logsumexp(logits[k, :]),
+ * in descending order, ties to the lowest k * V + v (inside a beam the order is that of
+ * the logits).  No counterpart in the reference, which picks greedily
+ * (src/llm_cuda/models/llama3/model.py:214); stands beside llmc_argmax.
+ *   logits: row g * K + k at logits + (g * K + k) * row_stride elements.
+ *   beam_scores [G, K] fp32; finished [G, K] bytes or NULL: a finished beam offers the
+ *     token eos at its own score and nothing else (its logits are not read).
+ *   A beam whose score, or whose log-sum-exp, is not finite (a NaN or +inf among its
+ *     logits, all of them -inf) offers its tokens at -inf.
+ *   out_scores [G, n] fp32, out_beams [G, n] int32 (0 .. K-1), out_tokens [G, n] int64.
+ * 1 <= K <= 32, 1 <= n <= 64, n <= K * V.  Ranked in fp64, scores rounded once to fp32.
+ * One launch, no workspace.
+ */
+LLMC_API int llmc_beam_select(const void* logits, long long row_stride, const float* beam_scores,
+                              const uint8_t* finished, float* out_scores, int32_t* out_beams,
+                              int64_t* out_tokens, int G, int K, int V, int n, int eos, int dtype,
+                              llmc_stream_t stream);
+
+/*
+ * Reordering of a paged cache after a beam selection, in place: beam i of a prompt becomes
+ * a continuation of beam parents[g, i].  No counterpart in the reference, whose cache holds
+ * one sequence (src/llm_cuda/models/llama3/kv_cache.py:6-36).
+ *   pools [layers, 2 (K, V), num_pages, Hkv, page_size, d], elem_bytes 2 or 4.
+ *   own_table [G * K, max_pages_per_seq] int32: the pages that beam b itself writes (and,
+ *     for the logical pages of its prompt, the prompt's).  Constant.  Behind the prompt
+ *     the rows name distinct pages.
+ *   block_table: the pages that a beam reads.  Row i takes the parent's entries below
+ *     logical page L / page_size and its own_table entries from there on.
+ *   seq_lens [G * K] int32: L, the same for all beams of a prompt; not written.
+ *   parents [G, K] int32, 0 .. K-1 within the prompt; repeats are allowed.
+ * The L % page_size tokens of the page in progress are copied from the parent's own page to
+ * the beam's, in every layer; full pages are shared, not copied.  A prompt with a bad
+ * parent or unequal lengths (LLMC_STATUS_BAD_PARENT), a bad own page or a bad length is
+ * left as it is.  1 <= K <= 32.  One launch.
+ */
+LLMC_API int llmc_beam_reorder(void* pools, const int32_t* own_table, int32_t* block_table,
+                               const int32_t* seq_lens, const int32_t* parents, int32_t* status,
+                               int G, int K, int layers, int Hkv, int d, int page_size,
+                               int max_pages_per_seq, int num_pages, int elem_bytes,
+                               llmc_stream_t stream);
 
 /*
  * Decode-step helpers around the attention path (config-5 decode loop).

@@ -26,6 +26,8 @@ STATUS_BITS = {
     4: "append past the cache capacity",
     8: "RoPE position outside the cos/sin table",
     16: "sequence length larger than the block table can address",
+    32: "sequence groups are not ascending ranges of the batch",
+    64: "beam parent outside its prompt, or beams of unequal length",
 }
 
 _DTYPE_CODE = {torch.float32: LLMC_F32, torch.float16: LLMC_F16, torch.bfloat16: LLMC_BF16}
@@ -59,6 +61,10 @@ SIGNATURES = {
     "llmc_ar_region_bytes": (_SZ, [_I, _I, _I, _I, ctypes.POINTER(_SZ)]),
     "llmc_allreduce_add_rmsnorm": (_I, [_P] * 8 + [_I] * 5 + [_F, _I, _P]),
     "llmc_argmax": (_I, [_P, _P, _I, _I, _I, _P, _P]),
+    "llmc_shared_prefix_workspace_bytes": (_SZ, [_I] * 8),
+    "llmc_shared_prefix_decode": (_I, [_P] * 9 + [_SZ, _P] + [_I] * 9 + [_F, _I, _I, _P]),
+    "llmc_beam_select": (_I, [_P, ctypes.c_longlong] + [_P] * 5 + [_I] * 6 + [_P]),
+    "llmc_beam_reorder": (_I, [_P] * 6 + [_I] * 9 + [_P]),
     "llmc_last_error_string": (ctypes.c_char_p, []),
     "llmc_version": (ctypes.c_char_p, []),
 }

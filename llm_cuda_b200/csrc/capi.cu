@@ -44,6 +44,23 @@ cudaError_t launch_swiglu(const void* gu, void* out, int rows, int inter, int dt
                           cudaStream_t stream);
 cudaError_t launch_argmax(const void* x, int64_t* out, int rows, int n, int dtype,
                           unsigned long long* keys, int* counters, int sms, cudaStream_t stream);
+size_t shared_prefix_workspace_bytes(int B, int Hq, int Hkv, int d, int P, int G, int max_group,
+                                     int dtype);
+cudaError_t launch_shared_prefix_decode(const void* q, const void* kp, const void* vp,
+                                        const int32_t* bt, const int32_t* seq_lens,
+                                        const int32_t* starts, const int32_t* shared, void* out,
+                                        float* ws, int32_t* status, int B, int Hq, int Hkv, int d,
+                                        int P, int max_pages, int num_pages, int G, int max_group,
+                                        float scale, int dtype, int flags, std::string* err,
+                                        cudaStream_t stream);
+cudaError_t launch_beam_select(const void* logits, long long row_stride, const float* beam_scores,
+                               const uint8_t* finished, float* out_scores, int32_t* out_beams,
+                               int64_t* out_tokens, int G, int K, int V, int n, int eos, int dtype,
+                               cudaStream_t stream);
+cudaError_t launch_beam_reorder(void* pools, const int32_t* own_table, int32_t* block_table,
+                                const int32_t* seq_lens, const int32_t* parents, int G, int K,
+                                int layers, int Hkv, int d, int P, int max_pages, int num_pages,
+                                int elem, int32_t* status, cudaStream_t stream);
 namespace ar {
 struct Params {
   const void* partial;
@@ -372,6 +389,112 @@ int llmc_argmax(const void* x, int64_t* out, int rows, int n, int dtype, void* w
   cudaError_t e = llmc::launch_argmax(x, out, rows, n, dtype, keys, counters,
                                       llmc::balanced_grid(), (cudaStream_t)stream);
   if (e != cudaSuccess) return cuda_fail(e, "llmc_argmax");
+  return LLMC_OK;
+}
+
+size_t llmc_shared_prefix_workspace_bytes(int B, int Hq, int Hkv, int d, int page_size,
+                                          int num_groups, int max_group, int dtype) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || d <= 0 || d > 256 || page_size <= 0 ||
+      num_groups < 0 || max_group < 1 || !valid_dtype(dtype))
+    return 0;
+  if (max_group > B) max_group = B;
+  return llmc::shared_prefix_workspace_bytes(B, Hq, Hkv, d, page_size, num_groups, max_group,
+                                             dtype);
+}
+
+int llmc_shared_prefix_decode(const void* q, const void* k_pages, const void* v_pages,
+                              const int32_t* block_table, const int32_t* seq_lens,
+                              const int32_t* group_starts, const int32_t* shared_lens, void* out,
+                              void* workspace, size_t workspace_bytes, int32_t* status, int B,
+                              int Hq, int Hkv, int d, int page_size, int max_pages_per_seq,
+                              int num_pages, int num_groups, int max_group, float scale, int dtype,
+                              int flags, llmc_stream_t stream) {
+  g_last_error.clear();
+  if (!valid_dtype(dtype)) return fail(LLMC_EINVAL, "llmc_shared_prefix_decode: unknown dtype");
+  if (B < 0 || Hq <= 0 || Hkv <= 0 || d <= 0 || page_size <= 0 || max_pages_per_seq <= 0 ||
+      num_pages <= 0 || num_groups < 0 || max_group < 1)
+    return fail(LLMC_EINVAL, "llmc_shared_prefix_decode: sizes must be positive");
+  if (Hq % Hkv)
+    return fail(LLMC_EINVAL, "llmc_shared_prefix_decode: Hq must be a multiple of Hkv");
+  if (d > 256) return fail(LLMC_EUNSUPPORTED, "llmc_shared_prefix_decode: head_dim > 256");
+  if ((long long)num_pages * Hkv * page_size >= (1ll << 31))
+    return fail(LLMC_EUNSUPPORTED, "llmc_shared_prefix_decode: page pool rows exceed 2^31");
+  if ((long long)max_pages_per_seq * page_size > INT_MAX)
+    return fail(LLMC_EINVAL,
+                "llmc_shared_prefix_decode: max_pages_per_seq * page_size exceeds 2^31-1");
+  if (max_group > B && B > 0) max_group = B;
+  if (!q || !k_pages || !v_pages || !block_table || !seq_lens || !out || !workspace || !status ||
+      (num_groups > 0 && (!group_starts || !shared_lens)))
+    return fail(LLMC_EINVAL, "llmc_shared_prefix_decode: NULL pointer argument");
+  if (reinterpret_cast<uintptr_t>(workspace) & 15)
+    return fail(LLMC_EINVAL, "llmc_shared_prefix_decode: workspace must be 16-byte aligned");
+  if (B == 0) return LLMC_OK;
+  if (num_groups > B)
+    return fail(LLMC_EINVAL, "llmc_shared_prefix_decode: more groups than sequences");
+  if (workspace_bytes < llmc::shared_prefix_workspace_bytes(B, Hq, Hkv, d, page_size, num_groups,
+                                                            max_group, dtype))
+    return fail(LLMC_EINVAL, "llmc_shared_prefix_decode: workspace too small");
+  std::string err;
+  cudaError_t e = llmc::launch_shared_prefix_decode(
+      q, k_pages, v_pages, block_table, seq_lens, group_starts, shared_lens, out,
+      static_cast<float*>(workspace), status, B, Hq, Hkv, d, page_size, max_pages_per_seq,
+      num_pages, num_groups, max_group, scale, dtype, flags, &err, (cudaStream_t)stream);
+  if (e == cudaErrorInvalidConfiguration && !err.empty())
+    return fail(LLMC_EUNSUPPORTED, "llmc_shared_prefix_decode: " + err);
+  if (e != cudaSuccess) return cuda_fail(e, "llmc_shared_prefix_decode", err);
+  return LLMC_OK;
+}
+
+int llmc_beam_select(const void* logits, long long row_stride, const float* beam_scores,
+                     const uint8_t* finished, float* out_scores, int32_t* out_beams,
+                     int64_t* out_tokens, int G, int K, int V, int n, int eos, int dtype,
+                     llmc_stream_t stream) {
+  g_last_error.clear();
+  if (!valid_dtype(dtype)) return fail(LLMC_EINVAL, "llmc_beam_select: unknown dtype");
+  if (G < 0 || G > (1 << 24) || K < 1 || K > 32 || V < 1)
+    return fail(LLMC_EINVAL, "llmc_beam_select: need 0 <= G <= 2^24, 1 <= K <= 32, V >= 1");
+  if (V > INT_MAX - 64) return fail(LLMC_EUNSUPPORTED, "llmc_beam_select: V too large");
+  if (n < 1 || n > 64 || (long long)n > (long long)K * V)
+    return fail(LLMC_EINVAL, "llmc_beam_select: need 1 <= n <= 64 and n <= K * V");
+  if (row_stride < V) return fail(LLMC_EINVAL, "llmc_beam_select: row_stride smaller than V");
+  if (finished && (eos < 0 || eos >= V))
+    return fail(LLMC_EINVAL, "llmc_beam_select: finished beams need 0 <= eos < V");
+  if (!logits || !beam_scores || !out_scores || !out_beams || !out_tokens)
+    return fail(LLMC_EINVAL, "llmc_beam_select: NULL pointer argument");
+  if (reinterpret_cast<uintptr_t>(logits) & (dtype == LLMC_F32 ? 3 : 1))
+    return fail(LLMC_EINVAL, "llmc_beam_select: misaligned logits");
+  if (G == 0) return LLMC_OK;
+  cudaError_t e = llmc::launch_beam_select(logits, row_stride, beam_scores, finished, out_scores,
+                                           out_beams, out_tokens, G, K, V, n, eos, dtype,
+                                           (cudaStream_t)stream);
+  if (e != cudaSuccess) return cuda_fail(e, "llmc_beam_select");
+  return LLMC_OK;
+}
+
+int llmc_beam_reorder(void* pools, const int32_t* own_table, int32_t* block_table,
+                      const int32_t* seq_lens, const int32_t* parents, int32_t* status, int G,
+                      int K, int layers, int Hkv, int d, int page_size, int max_pages_per_seq,
+                      int num_pages, int elem_bytes, llmc_stream_t stream) {
+  g_last_error.clear();
+  if (elem_bytes != 2 && elem_bytes != 4)
+    return fail(LLMC_EINVAL, "llmc_beam_reorder: elem_bytes must be 2 or 4");
+  if (G < 0 || G > 65535 || K < 1 || K > 32)
+    return fail(LLMC_EINVAL, "llmc_beam_reorder: need 0 <= G <= 65535 and 1 <= K <= 32");
+  if (layers < 1 || Hkv < 1 || d < 1 || page_size < 1 || max_pages_per_seq < 1 || num_pages < 1)
+    return fail(LLMC_EINVAL, "llmc_beam_reorder: sizes must be positive");
+  if ((long long)page_size * d * elem_bytes * Hkv > INT_MAX)
+    return fail(LLMC_EUNSUPPORTED, "llmc_beam_reorder: a page exceeds 2^31-1 bytes");
+  if ((long long)max_pages_per_seq * page_size > INT_MAX)
+    return fail(LLMC_EINVAL, "llmc_beam_reorder: max_pages_per_seq * page_size exceeds 2^31-1");
+  if (!pools || !own_table || !block_table || !seq_lens || !parents || !status)
+    return fail(LLMC_EINVAL, "llmc_beam_reorder: NULL pointer argument");
+  if (own_table == block_table)
+    return fail(LLMC_EINVAL, "llmc_beam_reorder: own_table and block_table must be two tables");
+  if (G == 0) return LLMC_OK;
+  cudaError_t e = llmc::launch_beam_reorder(pools, own_table, block_table, seq_lens, parents, G, K,
+                                            layers, Hkv, d, page_size, max_pages_per_seq,
+                                            num_pages, elem_bytes, status, (cudaStream_t)stream);
+  if (e != cudaSuccess) return cuda_fail(e, "llmc_beam_reorder");
   return LLMC_OK;
 }
 

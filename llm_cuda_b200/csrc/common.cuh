@@ -30,6 +30,8 @@ enum StatusBits : int {
   kStatusAppendOverflow = 4,   // append past max_pages_per_seq * page_size
   kStatusRopeRange = 8,        // RoPE position outside the cos/sin table
   kStatusSeqLenRange = 16,     // seq_len larger than the block table can address
+  kStatusBadGroup = 32,        // sequence groups that are not ascending ranges of the batch
+  kStatusBadParent = 64,       // a beam's parent outside its prompt, or beams of unequal length
 };
 
 // Every bounded wait gives up after this many nanoseconds of %globaltimer.

@@ -1,0 +1,288 @@
+// Single-token decode attention for a batch whose sequences share prefixes, paged K/V.
+//
+//   out[b, h] = softmax_t(q[b, h] . k_t * scale) . v_t   over the seq_lens[b] tokens of b
+//
+// For a group of n sequences with a common prefix of s tokens, the n * R query rows that
+// use one KV head (R = query heads per KV head) meet the same s keys and values: one
+// matrix product that reads them once, where separate sequences read them n times.  The
+// tokens behind the prefix are a sequence's own.  Both parts leave a normalised partial
+// and its log2-sum-exp per row, and the parts are joined by
+//   M = max lse_i,  out = sum 2^(lse_i - M) o_i / sum 2^(lse_i - M).
+// Scores, maxima, sums and partials are fp32; only out is rounded to the tensor type.
+//
+// The kernels of this file take every type, head size and page size: shared-prefix rows
+// and own rows alike are cut into units of 16 query rows x a range of tokens, in fp32 on
+// the CUDA cores, with 32 tokens of K and V at a time in shared memory.
+#include <climits>
+#include <string>
+
+#include "shared_prefix.cuh"
+
+namespace llmc {
+namespace prefix {
+namespace generic {
+
+constexpr int kRows = 16;     // query rows of a unit
+constexpr int kTok = 32;      // tokens per step
+constexpr int kThreads = 256; // 16 threads per row
+
+__host__ __device__ inline size_t smem_bytes(int d) {
+  return sizeof(float) * ((size_t)kRows * d + (size_t)kTok * (d + 1) + (size_t)kTok * d +
+                          kRows * (kTok + 1));
+}
+
+// Partials: part_o [2 * nsplit][B * Hq][d], part_lse [2 * nsplit][B * Hq]; slots below
+// nsplit are the shared part's, the others the own part's.
+// Grid: x = split, y = unit of a KV head, z = KV head.  Units: the tiles of the groups'
+// rows (tiles of a group are sized for max_group), then the tiles of every sequence.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) units_kernel(const Params p, int group_tiles,
+                                                         int seq_tiles) {
+  extern __shared__ float sm[];
+  __shared__ int scratch[2];
+  const int d = p.d;
+  float* Qs = sm;                              // [16][d]
+  float* Ks = Qs + kRows * d;                  // [32][d + 1]
+  float* Vs = Ks + kTok * (d + 1);             // [32][d]
+  float* Ps = Vs + kTok * d;                   // [16][33]
+  const int split = blockIdx.x, hk = blockIdx.z;
+  const bool is_group = (int)blockIdx.y < p.G * group_tiles;
+  const int tid = threadIdx.x;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  int lo, nrows, row0, t_begin, t_end, table_row;
+  if (is_group) {
+    const int g = blockIdx.y / group_tiles, tile = blockIdx.y % group_tiles;
+    int hi, s, leader;
+    group_range(p, g, lo, hi);
+    row0 = tile * kRows;
+    nrows = (hi - lo) * p.R;
+    if (row0 >= nrows) return;
+    group_prefix(p, g, lo, hi, scratch, s, leader);
+    if (s == 0) return;            // the sequences' own units mark the shared slots empty
+    t_begin = 0;
+    t_end = s;
+    table_row = leader;
+  } else {
+    const int u = blockIdx.y - p.G * group_tiles;
+    lo = u / seq_tiles;
+    row0 = (u % seq_tiles) * kRows;
+    nrows = p.R;
+    const int g = group_of(p, lo, scratch);
+    int s = 0;
+    if (g >= 0) {
+      int glo, ghi, leader;
+      group_range(p, g, glo, ghi);
+      group_prefix(p, g, glo, ghi, scratch, s, leader);
+    }
+    t_end = seq_len(p, lo, split == 0 && tid == 0);
+    t_begin = min(s, t_end);
+    table_row = lo;
+    if (t_begin == 0 && tid < kRows && row0 + tid < nrows)   // no shared part
+      p.part_lse[((long long)split * p.B + lo) * p.Hq + hk * p.R + row0 + tid] =
+          __int_as_float(0xff800000);
+  }
+  // this block's share of the tokens, in whole steps
+  const int steps = (t_end - t_begin + kTok - 1) / kTok;
+  const int s0 = (int)((long long)steps * split / p.nsplit);
+  const int s1 = (int)((long long)steps * (split + 1) / p.nsplit);
+  const int first = t_begin + s0 * kTok, last = min(t_end, t_begin + s1 * kTok);
+
+  const int r = tid >> 4, c = tid & 15;
+  const int row = row0 + r;                       // row of the unit's row set
+  const int b = lo + row / p.R, h = hk * p.R + row % p.R;
+  const bool valid = row < nrows;
+  const T* q = reinterpret_cast<const T*>(p.q);
+  for (int i = c; i < d; i += 16)
+    Qs[r * d + i] = valid ? to_f32(q[((long long)b * p.Hq + h) * d + i]) * p.scale_log2 : 0.f;
+
+  const T* kp = reinterpret_cast<const T*>(p.k_pages);
+  const T* vp = reinterpret_cast<const T*>(p.v_pages);
+  const float kNegInf = __int_as_float(0xff800000);
+  float m = kNegInf, l = 0.f, acc[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) acc[j] = 0.f;
+
+  for (int t0 = first; t0 < last; t0 += kTok) {
+    const int nt = min(kTok, last - t0);
+    __syncthreads();
+    // 8 threads per token load its key and value
+    {
+      const int t = tid >> 3;
+      if (t < nt) {
+        const int tok = t0 + t;
+        const long long base =
+            (((long long)page_of(p, table_row, tok) * p.Hkv + hk) * p.P + tok % p.P) * d;
+        for (int i = tid & 7; i < d; i += 8) {
+          Ks[t * (d + 1) + i] = to_f32(kp[base + i]);
+          Vs[t * d + i] = to_f32(vp[base + i]);
+        }
+      } else {
+        for (int i = tid & 7; i < d; i += 8) {
+          Ks[t * (d + 1) + i] = 0.f;
+          Vs[t * d + i] = 0.f;
+        }
+      }
+    }
+    __syncthreads();
+    float x0 = 0.f, x1 = 0.f;
+    for (int i = 0; i < d; ++i) {
+      const float qv = Qs[r * d + i];
+      x0 = fmaf(qv, Ks[c * (d + 1) + i], x0);
+      x1 = fmaf(qv, Ks[(c + 16) * (d + 1) + i], x1);
+    }
+    if (c >= nt) x0 = kNegInf;
+    if (c + 16 >= nt) x1 = kNegInf;
+    float tm = fmaxf(x0, x1);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
+    const float mn = fmaxf(m, tm);
+    const float mu = mn == kNegInf ? 0.f : mn;    // every score -inf: weights 0
+    const float f = exp2f(m - mu);
+    const float p0 = exp2f(x0 - mu), p1 = exp2f(x1 - mu);
+    float ps = p0 + p1;
+#pragma unroll
+    for (int o = 8; o; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
+    l = l * f + ps;
+    m = mn;
+    Ps[r * (kTok + 1) + c] = p0;
+    Ps[r * (kTok + 1) + c + 16] = p1;
+    __syncwarp();                                 // a row's threads are in one warp
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[j] *= f;
+    for (int t = 0; t < nt; ++t) {
+      const float w = Ps[r * (kTok + 1) + t];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (c + 16 * j < d) acc[j] = fmaf(w, Vs[t * d + c + 16 * j], acc[j]);
+    }
+  }
+  if (!valid) return;
+  const int slot = (is_group ? 0 : p.nsplit) + split;
+  const long long o = ((long long)slot * p.B + b) * p.Hq + h;
+  // An empty sequence has no part in its group's prefix.
+  const bool none = l == 0.f || (is_group && p.seq_lens[b] <= 0);
+  const float inv = none ? 0.f : 1.f / l;
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    if (c + 16 * j < d) p.part_o[o * d + c + 16 * j] = none ? 0.f : acc[j] * inv;
+  if (c == 0) p.part_lse[o] = none ? kNegInf : m + log2f(l);
+}
+
+// One warp per row (b, h).
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const Params p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long rows = (long long)p.B * p.Hq;
+  const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const int n = 2 * p.nsplit;
+  float M = __int_as_float(0xff800000);
+  for (int i = 0; i < n; ++i) M = fmaxf(M, p.part_lse[i * rows + row]);
+  float acc[8], L = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+  for (int i = 0; i < n; ++i) {
+    const float lse = p.part_lse[i * rows + row];
+    if (lse == __int_as_float(0xff800000)) continue;   // nothing in this part
+    const float w = exp2f(lse - M);
+    L += w;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (lane + 32 * j < p.d)
+        acc[j] = fmaf(w, p.part_o[(i * rows + row) * p.d + lane + 32 * j], acc[j]);
+  }
+  T* out = reinterpret_cast<T*>(p.out) + row * p.d;
+  const float inv = L > 0.f ? 1.f / L : L != L ? L : 0.f;   // an empty sequence gives zeros
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (lane + 32 * j < p.d) out[lane + 32 * j] = from_f32<T>(acc[j] * inv);
+}
+
+}  // namespace generic
+}  // namespace prefix
+
+static int generic_splits(int B, int Hq, int Hkv, int G, int max_group) {
+  // Splits of a unit's tokens: enough blocks for four per SM, at most 16.
+  const int R = Hq / Hkv;
+  const long long units = (long long)Hkv * ((long long)G * (((long long)max_group * R + 15) / 16) +
+                                            (long long)B * ((R + 15) / 16));
+  long long s = (4 * 148 + units - 1) / units;
+  return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
+}
+
+size_t shared_prefix_workspace_bytes(int B, int Hq, int Hkv, int d, int P, int G, int max_group,
+                                     int dtype) {
+  (void)P; (void)dtype;
+  const int s = generic_splits(B, Hq, Hkv, G, max_group);
+  return (size_t)2 * s * B * Hq * ((size_t)d + 1) * sizeof(float);
+}
+
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_chained(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
+                                  cudaStream_t stream, Args... args) {
+  if (smem > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t launch_generic(prefix::Params p, float* ws, cudaStream_t stream) {
+  namespace gen = prefix::generic;
+  const int group_tiles = (int)(((long long)p.max_group * p.R + gen::kRows - 1) / gen::kRows);
+  const int seq_tiles = (p.R + gen::kRows - 1) / gen::kRows;
+  p.nsplit = generic_splits(p.B, p.Hq, p.Hkv, p.G, p.max_group);
+  p.part_o = ws;
+  p.part_lse = ws + (size_t)2 * p.nsplit * p.B * p.Hq * p.d;
+  const long long units = (long long)p.G * group_tiles + (long long)p.B * seq_tiles;
+  if (units > 65535 || p.Hkv > 65535) return cudaErrorInvalidConfiguration;
+  cudaError_t e = launch_chained(gen::units_kernel<T>, dim3(p.nsplit, (unsigned)units, p.Hkv),
+                                 dim3(gen::kThreads), gen::smem_bytes(p.d), stream, p,
+                                 group_tiles, seq_tiles);
+  if (e != cudaSuccess) return e;
+  const long long rows = (long long)p.B * p.Hq;
+  return launch_chained(gen::join_kernel<T>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0,
+                        stream, p);
+}
+
+cudaError_t launch_shared_prefix_decode(const void* q, const void* kp, const void* vp,
+                                        const int32_t* bt, const int32_t* seq_lens,
+                                        const int32_t* starts, const int32_t* shared, void* out,
+                                        float* ws, int32_t* status, int B, int Hq, int Hkv, int d,
+                                        int P, int max_pages, int num_pages, int G, int max_group,
+                                        float scale, int dtype, int flags, std::string* err,
+                                        cudaStream_t stream) {
+  prefix::Params p;
+  p.q = q; p.k_pages = kp; p.v_pages = vp; p.block_table = bt; p.seq_lens = seq_lens;
+  p.starts = starts; p.shared = shared; p.out = out; p.status = status;
+  p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.R = Hq / Hkv; p.d = d; p.P = P; p.max_pages = max_pages;
+  p.num_pages = num_pages; p.G = G; p.max_group = max_group;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  (void)flags;
+  cudaError_t e;
+  if (dtype == LLMC_F32) e = launch_generic<float>(p, ws, stream);
+  else if (dtype == LLMC_F16) e = launch_generic<__half>(p, ws, stream);
+  else e = launch_generic<__nv_bfloat16>(p, ws, stream);
+  if (e == cudaErrorInvalidConfiguration)
+    *err = "more than 65535 row tiles (groups x max_group, sequences) for this shape";
+  return e;
+}
+
+}  // namespace llmc

@@ -1,0 +1,86 @@
+"""Refusals of the beam and shared-prefix entry points, before any launch (no GPU)."""
+
+import pytest
+import torch
+
+import llm_cuda_b200._native as N
+from llm_cuda_b200.kernels.beam import beam_reorder, beam_select
+from llm_cuda_b200.kernels.shared_prefix import shared_prefix_decode
+
+
+def _prefix(lib, q=16, ws=16, nbytes=1 << 40, B=4, Hq=8, Hkv=2, d=128, P=16, mp=4, np_=8, G=1,
+            mg=4, dt=N.LLMC_BF16):
+    return lib.llmc_shared_prefix_decode(q, 16, 16, 16, 16, 16, 16, 16, ws, nbytes, 16, B, Hq, Hkv,
+                                         d, P, mp, np_, G, mg, 0.1, dt, 0, None)
+
+
+def test_shared_prefix_refusals():
+    lib = N.load()
+    err = lib.llmc_last_error_string
+    assert _prefix(lib, dt=9) == -1 and b"dtype" in err()
+    assert _prefix(lib, Hkv=3) == -1 and b"multiple" in err()
+    assert _prefix(lib, d=257) == -2
+    assert _prefix(lib, q=None) == -1 and b"NULL" in err()
+    assert _prefix(lib, ws=20) == -1 and b"aligned" in err()
+    assert _prefix(lib, nbytes=16) == -1 and b"workspace" in err()
+    assert _prefix(lib, mg=0) == -1
+    assert _prefix(lib, G=5) == -1 and b"groups" in err()
+    assert _prefix(lib, mp=1 << 28, P=16) == -1
+    assert _prefix(lib, np_=1 << 28) == -2
+    assert _prefix(lib, B=0) == 0
+    need = lib.llmc_shared_prefix_workspace_bytes(4, 8, 2, 128, 16, 1, 4, N.LLMC_BF16)
+    assert need > 0
+    assert lib.llmc_shared_prefix_workspace_bytes(4, 8, 2, 128, 16, 1, 400, N.LLMC_BF16) == need
+    assert lib.llmc_shared_prefix_workspace_bytes(4, 7, 2, 128, 16, 1, 4, N.LLMC_BF16) == 0
+
+
+def _select(lib, logits=16, stride=100, G=1, K=4, V=100, n=4, eos=-1, fin=None, dt=N.LLMC_BF16):
+    return lib.llmc_beam_select(logits, stride, 16, fin, 16, 16, 16, G, K, V, n, eos, dt, None)
+
+
+def test_beam_select_refusals():
+    lib = N.load()
+    err = lib.llmc_last_error_string
+    assert _select(lib, dt=5) == -1 and b"dtype" in err()
+    assert _select(lib, K=33) == -1
+    assert _select(lib, K=0) == -1
+    assert _select(lib, n=65) == -1 and b"n <= 64" in err()
+    assert _select(lib, V=1, stride=1, n=5) == -1
+    assert _select(lib, stride=99) == -1 and b"row_stride" in err()
+    assert _select(lib, fin=16) == -1 and b"eos" in err()
+    assert _select(lib, fin=16, eos=100) == -1
+    assert _select(lib, logits=17) == -1 and b"misaligned" in err()
+    assert _select(lib, logits=18, dt=N.LLMC_F32) == -1
+    assert _select(lib, logits=None) == -1
+    assert _select(lib, G=0) == 0
+
+
+def _reorder(lib, pools=16, own=16, bt=32, G=1, K=4, layers=2, Hkv=2, d=64, P=16, mp=4, np_=8, e=2):
+    return lib.llmc_beam_reorder(pools, own, bt, 16, 16, 16, G, K, layers, Hkv, d, P, mp, np_, e,
+                                 None)
+
+
+def test_beam_reorder_refusals():
+    lib = N.load()
+    err = lib.llmc_last_error_string
+    assert _reorder(lib, e=1) == -1 and b"elem_bytes" in err()
+    assert _reorder(lib, K=33) == -1
+    assert _reorder(lib, G=65536) == -1
+    assert _reorder(lib, layers=0) == -1
+    assert _reorder(lib, bt=16) == -1 and b"two tables" in err()
+    assert _reorder(lib, pools=None) == -1
+    assert _reorder(lib, P=1 << 20, d=1 << 10) == -2
+    assert _reorder(lib, P=1 << 20, d=1, mp=1 << 12) == -1
+    assert _reorder(lib, G=0) == 0
+
+
+def test_python_entry_points_refuse_cpu_tensors():
+    q = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
+    kv = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        shared_prefix_decode(q, kv, kv, i.view(2, 1), i, i, i[:1])
+    with pytest.raises(ValueError, match="CUDA"):
+        beam_select(torch.zeros(2, 10), torch.zeros(1, 2))
+    with pytest.raises(ValueError, match="CUDA"):
+        beam_reorder(torch.zeros(1, 2, 4, 2, 16, 64), i.view(2, 1), i.view(2, 1), i, i.view(1, 2))
