@@ -10,13 +10,15 @@
 //   M = max lse_i,  out = sum 2^(lse_i - M) o_i / sum 2^(lse_i - M).
 // Scores, maxima, sums and partials are fp32; only out is rounded to the tensor type.
 //
-// The kernels of this file take every type, head size and page size: shared-prefix rows
-// and own rows alike are cut into units of 16 query rows x a range of tokens, in fp32 on
-// the CUDA cores, with 32 tokens of K and V at a time in shared memory.
+// bf16/fp16 at head size 64 or 128 and pages of 8, 16, 32, 64 or a multiple of 128 tokens
+// run on the tensor cores (shared_prefix_tc.cuh).  The kernels of this file take every
+// other type, head size and page size: shared-prefix rows and own rows alike are cut into
+// units of 16 query rows x a range of tokens, in fp32 on the CUDA cores, with 32 tokens of
+// K and V at a time in shared memory.
 #include <climits>
 #include <string>
 
-#include "shared_prefix.cuh"
+#include "shared_prefix_tc.cuh"
 
 namespace llmc {
 namespace prefix {
@@ -205,7 +207,21 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
 }  // namespace generic
 }  // namespace prefix
 
-static int generic_splits(int B, int Hq, int Hkv, int G, int max_group) {
+namespace {
+struct Device {
+  int sms = 0, smem = 0;
+};
+Device device() {
+  Device d;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
+  cudaDeviceGetAttribute(&d.smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+  if (d.sms <= 0) d.sms = 148;   // no device (sizes are asked for on the host): a B200
+  return d;
+}
+
+int generic_splits(int B, int Hq, int Hkv, int G, int max_group) {
   // Splits of a unit's tokens: enough blocks for four per SM, at most 16.
   const int R = Hq / Hkv;
   const long long units = (long long)Hkv * ((long long)G * (((long long)max_group * R + 15) / 16) +
@@ -214,37 +230,90 @@ static int generic_splits(int B, int Hq, int Hkv, int G, int max_group) {
   return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
 }
 
-size_t shared_prefix_workspace_bytes(int B, int Hq, int Hkv, int d, int P, int G, int max_group,
-                                     int dtype) {
-  (void)P; (void)dtype;
+size_t generic_workspace(int B, int Hq, int Hkv, int d, int G, int max_group) {
   const int s = generic_splits(B, Hq, Hkv, G, max_group);
   return (size_t)2 * s * B * Hq * ((size_t)d + 1) * sizeof(float);
 }
 
+// Workspace of the tensor-core kernels: plan, then part_o, then part_lse.
+struct TcSizes {
+  size_t plan, part_o, part_lse;
+  int rs_a, rs_b;
+};
+TcSizes tc_sizes(int B, int R, int Hkv, int d, int G, int max_group, int ctas) {
+  TcSizes z;
+  const long long rows = (long long)max_group * R;
+  z.rs_a = (int)((rows < 128 ? rows : 128) + 31) / 32 * 32;
+  z.rs_b = 256;
+  // A group has at most ceil(rows / tile) row tiles: over all groups, B R / tile + G.
+  const size_t slots_a = ((size_t)((long long)B * R / 128) + G) * Hkv + ctas;
+  const size_t slots_b = rows > 128 ? ((size_t)((long long)B * R / 256) + G) * Hkv + ctas : 0;
+  const size_t a = slots_a * z.rs_a, b = slots_b * z.rs_b;
+  const size_t most = a > b ? a : b;
+  z.plan = ((size_t)8 + 4 * (size_t)G) * sizeof(int32_t);
+  z.plan = (z.plan + 255) / 256 * 256;
+  z.part_o = most * (size_t)d * sizeof(float);
+  z.part_lse = most * sizeof(float);
+  return z;
+}
+
+bool tc_shape(int dtype, int d, int P, int max_pages, int B, int Hq, int Hkv, int G) {
+  if (dtype != LLMC_BF16 && dtype != LLMC_F16) return false;
+  if (d != 64 && d != 128) return false;
+  if (!(P == 8 || P == 16 || P == 32 || P == 64 || P % 128 == 0)) return false;
+  if (G > prefix::tc::kMaxGroups || B > 65535) return false;
+  const long long R = Hq / Hkv;
+  if ((long long)Hkv * ((R + 7) / 8) > 65535) return false;
+  // chunk numbers are 32-bit
+  const long long chunks = ((long long)B * R / 128 + G) * Hkv *
+                           (((long long)max_pages * P + 127) / 128);
+  return chunks < (1ll << 31);
+}
+}  // namespace
+
+size_t shared_prefix_workspace_bytes(int B, int Hq, int Hkv, int d, int P, int G, int max_group,
+                                     int dtype) {
+  const size_t gen = generic_workspace(B, Hq, Hkv, d, G, max_group);
+  if (!tc_shape(dtype, d, P, 1, B, Hq, Hkv, G)) return gen;
+  const TcSizes z = tc_sizes(B, Hq / Hkv, Hkv, d, G, max_group, device().sms);
+  const size_t tc = z.plan + z.part_o + z.part_lse;
+  return tc > gen ? tc : gen;
+}
+
 template <typename... KArgs, typename... Args>
 static cudaError_t launch_chained(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                                  cudaStream_t stream, Args... args) {
+                                  int cluster, bool early, cudaStream_t stream, Args... args) {
   if (smem > 48 * 1024) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
     if (e != cudaSuccess) return e;
   }
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (early) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = n;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 template <typename T>
-static cudaError_t launch_generic(prefix::Params p, float* ws, cudaStream_t stream) {
+static cudaError_t launch_generic(prefix::Params p, float* ws, std::string* err,
+                                  cudaStream_t stream) {
   namespace gen = prefix::generic;
   const int group_tiles = (int)(((long long)p.max_group * p.R + gen::kRows - 1) / gen::kRows);
   const int seq_tiles = (p.R + gen::kRows - 1) / gen::kRows;
@@ -252,14 +321,98 @@ static cudaError_t launch_generic(prefix::Params p, float* ws, cudaStream_t stre
   p.part_o = ws;
   p.part_lse = ws + (size_t)2 * p.nsplit * p.B * p.Hq * p.d;
   const long long units = (long long)p.G * group_tiles + (long long)p.B * seq_tiles;
-  if (units > 65535 || p.Hkv > 65535) return cudaErrorInvalidConfiguration;
+  if (units > 65535 || p.Hkv > 65535) {
+    *err = "more than 65535 row tiles (groups x max_group, sequences) for this shape";
+    return cudaErrorInvalidConfiguration;
+  }
   cudaError_t e = launch_chained(gen::units_kernel<T>, dim3(p.nsplit, (unsigned)units, p.Hkv),
-                                 dim3(gen::kThreads), gen::smem_bytes(p.d), stream, p,
+                                 dim3(gen::kThreads), gen::smem_bytes(p.d), 1, true, stream, p,
                                  group_tiles, seq_tiles);
   if (e != cudaSuccess) return e;
   const long long rows = (long long)p.B * p.Hq;
-  return launch_chained(gen::join_kernel<T>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0,
-                        stream, p);
+  return launch_chained(gen::join_kernel<T>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, 1,
+                        true, stream, p);
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The pool as rows of d elements, boxes of 64 columns x `box` rows (a page or part of one).
+static bool encode_pool(CUtensorMap* map, const void* base, long long rows, int d, int box,
+                        int dtype, std::string* err) {
+  static EncodeTiledFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<EncodeTiledFn>(ptr);
+    return (EncodeTiledFn) nullptr;
+  }();
+  if (!fn) {
+    *err = "cuTensorMapEncodeTiled is not available";
+    return false;
+  }
+  cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)d * 2};
+  cuuint32_t boxd[2] = {64u, (cuuint32_t)box};
+  cuuint32_t estr[2] = {1u, 1u};
+  const CUresult r =
+      fn(map, dtype == LLMC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+         2, const_cast<void*>(base), dims, strides, boxd, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    *err = "cuTensorMapEncodeTiled failed with CUresult " + std::to_string((int)r);
+    return false;
+  }
+  return true;
+}
+
+template <int D, typename T>
+static cudaError_t launch_tc(const prefix::Params& p0, void* ws, int dtype, std::string* err,
+                             cudaStream_t stream) {
+  namespace tc = prefix::tc;
+  const Device di = device();
+  tc::TcParams tp;
+  tp.p = p0;
+  prefix::Params& p = tp.p;
+  const TcSizes z = tc_sizes(p.B, p.R, p.Hkv, D, p.G, p.max_group, di.sms);
+  tp.plan = static_cast<int32_t*>(ws);
+  p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + z.plan);
+  p.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + z.plan + z.part_o);
+  tp.rs_a = z.rs_a;
+  tp.rs_b = z.rs_b;
+  tp.ctas = di.sms;
+  if (p.G > 0) {
+    CUtensorMap mk, mv;
+    const long long rows = (long long)p.num_pages * p.Hkv * p.P;
+    const int box = p.P < tc::kChunk ? p.P : tc::kChunk;
+    if (!encode_pool(&mk, p.k_pages, rows, D, box, dtype, err) ||
+        !encode_pool(&mv, p.v_pages, rows, D, box, dtype, err))
+      return cudaErrorInvalidValue;
+    const size_t smem = tc::Smem<D>::bytes(p.G);
+    if (smem > (size_t)di.smem) {
+      *err = "not enough shared memory for the prefix pipeline";
+      return cudaErrorInvalidValue;
+    }
+    cudaError_t e = launch_chained(tc::prefix_kernel<D, T>, dim3(di.sms), dim3(tc::kThreads), smem,
+                                   1, true, stream, mk, mv, tp);
+    if (e != cudaSuccess) return e;
+  }
+  // Token splits of a sequence: a cluster of up to 8 blocks while the GPU has room for them.
+  const int nh = p.R > 8 ? 2 : 1;
+  const int hgs = (p.R + 8 * nh - 1) / (8 * nh);
+  const long long blocks = (long long)p.B * p.Hkv * hgs;
+  int ns = 1;
+  while (ns < 8 && blocks * ns * 2 <= 3ll * di.sms) ns *= 2;
+  const dim3 grid(ns, (unsigned)(p.Hkv * hgs), p.B);
+  // Without a prefix launch in front of it the own kernel has nothing to overlap with, and
+  // what it reads early would not be ordered behind earlier kernels.
+  return nh == 2 ? launch_chained(tc::own_kernel<D, 2, T>, grid, dim3(128), 0, ns, p.G > 0, stream, tp)
+                 : launch_chained(tc::own_kernel<D, 1, T>, grid, dim3(128), 0, ns, p.G > 0, stream, tp);
 }
 
 cudaError_t launch_shared_prefix_decode(const void* q, const void* kp, const void* vp,
@@ -272,17 +425,22 @@ cudaError_t launch_shared_prefix_decode(const void* q, const void* kp, const voi
   prefix::Params p;
   p.q = q; p.k_pages = kp; p.v_pages = vp; p.block_table = bt; p.seq_lens = seq_lens;
   p.starts = starts; p.shared = shared; p.out = out; p.status = status;
+  p.part_o = nullptr; p.part_lse = nullptr;
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.R = Hq / Hkv; p.d = d; p.P = P; p.max_pages = max_pages;
-  p.num_pages = num_pages; p.G = G; p.max_group = max_group;
+  p.num_pages = num_pages; p.G = G; p.max_group = max_group; p.nsplit = 1;
   p.scale_log2 = scale * 1.4426950408889634f;
-  (void)flags;
-  cudaError_t e;
-  if (dtype == LLMC_F32) e = launch_generic<float>(p, ws, stream);
-  else if (dtype == LLMC_F16) e = launch_generic<__half>(p, ws, stream);
-  else e = launch_generic<__nv_bfloat16>(p, ws, stream);
-  if (e == cudaErrorInvalidConfiguration)
-    *err = "more than 65535 row tiles (groups x max_group, sequences) for this shape";
-  return e;
+  auto al = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
+  if (!(flags & LLMC_DECODE_FORCE_GENERIC) && tc_shape(dtype, d, P, max_pages, B, Hq, Hkv, G) &&
+      al(q) && al(kp) && al(vp) && al(out)) {
+    if (dtype == LLMC_BF16)
+      return d == 128 ? launch_tc<128, __nv_bfloat16>(p, ws, dtype, err, stream)
+                      : launch_tc<64, __nv_bfloat16>(p, ws, dtype, err, stream);
+    return d == 128 ? launch_tc<128, __half>(p, ws, dtype, err, stream)
+                    : launch_tc<64, __half>(p, ws, dtype, err, stream);
+  }
+  if (dtype == LLMC_F32) return launch_generic<float>(p, ws, err, stream);
+  if (dtype == LLMC_F16) return launch_generic<__half>(p, ws, err, stream);
+  return launch_generic<__nv_bfloat16>(p, ws, err, stream);
 }
 
 }  // namespace llmc

@@ -289,3 +289,60 @@ def test_bad_inputs_set_the_status_word():
     b.run()
     with pytest.raises(N.DeviceStatusError, match="length"):
         N.raise_on_status(b.status)
+
+
+@pytest.mark.parametrize("n,L,hq,hkv,d,P,dtype", [
+    (40, 40007, 16, 2, 128, 64, BF), (9, 70001, 64, 2, 64, 16, HF), (37, 131072, 8, 1, 128, 256, BF)])
+def test_long_prefix_with_wide_row_tiles(n, L, hq, hkv, d, P, dtype):
+    """Enough work that a row tile has 256 rows; the 64-bit side runs on the GPU, the bound
+    is the one above."""
+    g = torch.Generator(device=DEV).manual_seed(L)
+    own = [i % 5 for i in range(n)]
+    full, f = L // P, L % P
+    pages = full + n * 2
+    kp = torch.randn(pages, hkv, P, d, device=DEV, generator=g).to(dtype)
+    vp = torch.randn(pages, hkv, P, d, device=DEV, generator=g).to(dtype)
+    bt = torch.full((n, full + 2), -1, dtype=torch.int32, device=DEV)
+    order = torch.randperm(pages, device=DEV, generator=g).to(torch.int32)
+    bt[:, :full] = order[:full]
+    bt[:, full:] = order[full:].view(n, 2)
+    ids = bt[:, full].long()
+    for pool in (kp, vp):
+        pool[ids, :, :f] = pool[ids[:1], :, :f].expand(n, -1, -1, -1)
+    q = torch.randn(n, hq, d, device=DEV, generator=g).to(dtype)
+    lens = torch.tensor([L + x for x in own], dtype=torch.int32, device=DEV)
+    st = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = shared_prefix_decode(q, kp, vp, bt, lens, torch.tensor([0, n], dtype=torch.int32, device=DEV),
+                               torch.tensor([L], dtype=torch.int32, device=DEV), status=st).double()
+    assert int(st.item()) == 0
+    u = torch.finfo(dtype).eps / 2
+    for b in range(0, n, 3):
+        m = L + own[b]
+        rows = bt[b, :-(-m // P)].long()
+        for h in range(hkv):
+            k = kp[rows, h].double().reshape(-1, d)[:m]
+            v = vp[rows, h].double().reshape(-1, d)[:m]
+            qs = q[b, h * (hq // hkv):(h + 1) * (hq // hkv)].double()
+            p = torch.softmax(qs @ k.T * d ** -0.5, -1)
+            o, A = p @ v, p @ v.abs()
+            e = (d + 4) * 2.0 ** -24 * (qs.abs() @ k.abs().T).amax(-1, keepdim=True) * d ** -0.5
+            tol = u * o.abs() + (u + 2 * e + 2 * 2.0 ** -21 + (2 * m + 16) * 2.0 ** -24) * A
+            bad = (out[b, h * (hq // hkv):(h + 1) * (hq // hkv)] - o).abs() / tol
+            assert float(bad.max()) <= 1.0
+
+
+def test_many_units_per_block():
+    """Every block works on several units in turn, each ending inside a chunk."""
+    lens0 = [300 + (613 * i) % 1749 for i in range(16)]
+    b = Batch([4] * 16, lens0, [x + 1 + (29 * i + j) % 128 for i, x in enumerate(lens0)
+                                for j in range(4)], 32, 8, 128, 16, BF, seed=13)
+    for _ in range(3):
+        b.check(b.run(max_group=4))
+
+
+def test_many_units_per_block_narrow_heads():
+    lens0 = [200 + (413 * i) % 1333 for i in range(40)]
+    b = Batch([3] * 40, lens0, [x + (29 * i + j) % 50 for i, x in enumerate(lens0)
+                                for j in range(3)], 16, 4, 64, 32, HF, seed=14)
+    for _ in range(3):
+        b.check(b.run(max_group=3))
