@@ -235,25 +235,28 @@ size_t generic_workspace(int B, int Hq, int Hkv, int d, int G, int max_group) {
   return (size_t)2 * s * B * Hq * ((size_t)d + 1) * sizeof(float);
 }
 
-// Workspace of the tensor-core kernels: plan, then part_o, then part_lse.
+// Workspace of the tensor-core kernels: plan, tables (if they do not fit shared memory),
+// partials of shared and of own units.
 struct TcSizes {
-  size_t plan, part_o, part_lse;
-  int rs_a, rs_b;
+  size_t plan, tables, o, lse, own_o, own_lse;
+  int nb, rs;
+  size_t total() const { return plan + tables + o + lse + own_o + own_lse; }
 };
-TcSizes tc_sizes(int B, int R, int Hkv, int d, int G, int max_group, int ctas) {
+size_t pad256(size_t x) { return (x + 255) / 256 * 256; }
+
+TcSizes tc_sizes(int B, int R, int Hkv, int d, int G, int max_group, const Device& di) {
   TcSizes z;
-  const long long rows = (long long)max_group * R;
-  z.rs_a = (int)((rows < 128 ? rows : 128) + 31) / 32 * 32;
-  z.rs_b = 256;
-  // A group has at most ceil(rows / tile) row tiles: over all groups, B R / tile + G.
-  const size_t slots_a = ((size_t)((long long)B * R / 128) + G) * Hkv + ctas;
-  const size_t slots_b = rows > 128 ? ((size_t)((long long)B * R / 256) + G) * Hkv + ctas : 0;
-  const size_t a = slots_a * z.rs_a, b = slots_b * z.rs_b;
-  const size_t most = a > b ? a : b;
-  z.plan = ((size_t)8 + 4 * (size_t)G) * sizeof(int32_t);
-  z.plan = (z.plan + 255) / 256 * 256;
-  z.part_o = most * (size_t)d * sizeof(float);
-  z.part_lse = most * sizeof(float);
+  z.nb = 128 / R < max_group ? 128 / R : max_group;
+  z.rs = z.nb * R;
+  // A group has at most ceil(rows / tile) row tiles: over all groups B / nb + G.
+  const size_t slots = 2 * (((size_t)(B / z.nb) + G) * Hkv + di.sms);
+  const size_t own = 2 * ((size_t)B * Hkv + di.sms);
+  z.plan = pad256((size_t)B * Hkv * sizeof(int4));
+  z.tables = pad256((prefix::tc::Tables::ints(G, B) + 4) * sizeof(int));
+  z.o = G ? pad256(slots * z.rs * d * sizeof(float)) : 0;
+  z.lse = G ? pad256(slots * z.rs * sizeof(float)) : 0;
+  z.own_o = pad256(own * R * d * sizeof(float));
+  z.own_lse = pad256(own * R * sizeof(float));
   return z;
 }
 
@@ -261,13 +264,12 @@ bool tc_shape(int dtype, int d, int P, int max_pages, int B, int Hq, int Hkv, in
   if (dtype != LLMC_BF16 && dtype != LLMC_F16) return false;
   if (d != 64 && d != 128) return false;
   if (!(P == 8 || P == 16 || P == 32 || P == 64 || P % 128 == 0)) return false;
-  if (G > prefix::tc::kMaxGroups || B > 65535) return false;
   const long long R = Hq / Hkv;
-  if ((long long)Hkv * ((R + 7) / 8) > 65535) return false;
-  // chunk numbers are 32-bit
-  const long long chunks = ((long long)B * R / 128 + G) * Hkv *
-                           (((long long)max_pages * P + 127) / 128);
-  return chunks < (1ll << 31);
+  if (R > 128) return false;
+  // chunk and slot numbers are 32-bit; a group's row tiles are of at least R rows
+  if ((long long)B * Hq >= (1ll << 31)) return false;
+  const long long units = 2ll * B * Hkv + (long long)G * Hkv;   // costs are up to 4 a chunk
+  return units * (((long long)max_pages * P + 127) / 128 + 1) < (1ll << 28);
 }
 }  // namespace
 
@@ -275,8 +277,8 @@ size_t shared_prefix_workspace_bytes(int B, int Hq, int Hkv, int d, int P, int G
                                      int dtype) {
   const size_t gen = generic_workspace(B, Hq, Hkv, d, G, max_group);
   if (!tc_shape(dtype, d, P, 1, B, Hq, Hkv, G)) return gen;
-  const TcSizes z = tc_sizes(B, Hq / Hkv, Hkv, d, G, max_group, device().sms);
-  const size_t tc = z.plan + z.part_o + z.part_lse;
+  const TcSizes z = tc_sizes(B, Hq / Hkv, Hkv, d, G, max_group, device());
+  const size_t tc = z.total();
   return tc > gen ? tc : gen;
 }
 
@@ -339,9 +341,9 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// The pool as rows of d elements, boxes of 64 columns x `box` rows (a page or part of one).
-static bool encode_pool(CUtensorMap* map, const void* base, long long rows, int d, int box,
-                        int dtype, std::string* err) {
+// A row-major tensor of 16-bit elements, 64-column boxes with 128-byte swizzle.
+static bool encode(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims,
+                   const cuuint64_t* strides, const cuuint32_t* box, int dtype, std::string* err) {
   static EncodeTiledFn fn = [] {
     void* ptr = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -355,20 +357,44 @@ static bool encode_pool(CUtensorMap* map, const void* base, long long rows, int 
     *err = "cuTensorMapEncodeTiled is not available";
     return false;
   }
-  cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)d * 2};
-  cuuint32_t boxd[2] = {64u, (cuuint32_t)box};
-  cuuint32_t estr[2] = {1u, 1u};
+  const cuuint32_t estr[3] = {1u, 1u, 1u};
   const CUresult r =
       fn(map, dtype == LLMC_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-         2, const_cast<void*>(base), dims, strides, boxd, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+         (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr,
+         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     *err = "cuTensorMapEncodeTiled failed with CUresult " + std::to_string((int)r);
     return false;
   }
   return true;
+}
+
+// The pool as rows of d elements; a box is a page or part of one.
+static bool encode_pool(CUtensorMap* map, const void* base, long long rows, int d, int box,
+                        int dtype, std::string* err) {
+  const cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)d * 2};
+  const cuuint32_t b[2] = {64u, (cuuint32_t)box};
+  return encode(map, base, 2, dims, strides, b, dtype, err);
+}
+
+// The same as [half][row][64 columns]: a box is a page of all its halves.
+static bool encode_pool_halves(CUtensorMap* map, const void* base, long long rows, int d, int box,
+                               int dtype, std::string* err) {
+  const cuuint64_t dims[3] = {64u, (cuuint64_t)rows, (cuuint64_t)(d / 64)};
+  const cuuint64_t strides[2] = {(cuuint64_t)d * 2, 128u};
+  const cuuint32_t b[3] = {64u, (cuuint32_t)box, (cuuint32_t)(d / 64)};
+  return encode(map, base, 3, dims, strides, b, dtype, err);
+}
+
+// q [B, Hq, d]; a box is the R heads of one KV head of nb sequences, in row order.
+static bool encode_q(CUtensorMap* map, const void* base, int B, int Hq, int d, int R, int nb,
+                     int dtype, std::string* err) {
+  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)Hq, (cuuint64_t)B};
+  const cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)Hq * d * 2};
+  const cuuint32_t b[3] = {64u, (cuuint32_t)R, (cuuint32_t)nb};
+  return encode(map, base, 3, dims, strides, b, dtype, err);
 }
 
 template <int D, typename T>
@@ -379,40 +405,49 @@ static cudaError_t launch_tc(const prefix::Params& p0, void* ws, int dtype, std:
   tc::TcParams tp;
   tp.p = p0;
   prefix::Params& p = tp.p;
-  const TcSizes z = tc_sizes(p.B, p.R, p.Hkv, D, p.G, p.max_group, di.sms);
-  tp.plan = static_cast<int32_t*>(ws);
-  p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + z.plan);
-  p.part_lse = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + z.plan + z.part_o);
-  tp.rs_a = z.rs_a;
-  tp.rs_b = z.rs_b;
+  const TcSizes z = tc_sizes(p.B, p.R, p.Hkv, D, p.G, p.max_group, di);
+  uint8_t* at = static_cast<uint8_t*>(ws);
+  tp.plan = reinterpret_cast<int4*>(at);
+  at += z.plan;
+  tp.heads = reinterpret_cast<int32_t*>(at);
+  tp.tables = tp.heads + 4;
+  at += z.tables;
+  p.part_o = reinterpret_cast<float*>(at);
+  at += z.o;
+  p.part_lse = reinterpret_cast<float*>(at);
+  at += z.lse;
+  tp.own_o = reinterpret_cast<float*>(at);
+  at += z.own_o;
+  tp.own_lse = reinterpret_cast<float*>(at);
+  tp.nb = z.nb;
+  tp.rs = z.rs;
   tp.ctas = di.sms;
-  if (p.G > 0) {
-    CUtensorMap mk, mv;
-    const long long rows = (long long)p.num_pages * p.Hkv * p.P;
-    const int box = p.P < tc::kChunk ? p.P : tc::kChunk;
-    if (!encode_pool(&mk, p.k_pages, rows, D, box, dtype, err) ||
-        !encode_pool(&mv, p.v_pages, rows, D, box, dtype, err))
-      return cudaErrorInvalidValue;
-    const size_t smem = tc::Smem<D>::bytes(p.G);
-    if (smem > (size_t)di.smem) {
-      *err = "not enough shared memory for the prefix pipeline";
-      return cudaErrorInvalidValue;
-    }
-    cudaError_t e = launch_chained(tc::prefix_kernel<D, T>, dim3(di.sms), dim3(tc::kThreads), smem,
-                                   1, true, stream, mk, mv, tp);
+  CUtensorMap mk, mv, mq, mq1;
+  const long long rows = (long long)p.num_pages * p.Hkv * p.P;
+  const int box = p.P < tc::kChunk ? p.P : tc::kChunk;
+  if (!encode_pool(&mk, p.k_pages, rows, D, box, dtype, err) ||
+      !encode_pool_halves(&mv, p.v_pages, rows, D, box, dtype, err) ||
+      !encode_q(&mq, p.q, p.B, p.Hq, D, p.R, z.nb, dtype, err) ||
+      !encode_q(&mq1, p.q, p.B, p.Hq, D, p.R, 1, dtype, err))
+    return cudaErrorInvalidValue;
+  // Tables in shared memory, unless the batch is too large for what the tiles leave.
+  const size_t fixed = 1024 + tc::Smem<D>::kTables;
+  const size_t tables = tc::Tables::ints(p.G, p.B) * sizeof(int);
+  cudaError_t e;
+  if (fixed + tables > (size_t)di.smem) {
+    e = launch_chained(tc::tables_kernel, dim3(1), dim3(1024), 0, 1, true, stream, tp);
     if (e != cudaSuccess) return e;
+    e = launch_chained(tc::parts_kernel<D, T, true>, dim3(di.sms), dim3(tc::kThreads), fixed, 1,
+                       true, stream, mk, mv, mq, mq1, tp);
+  } else {
+    e = launch_chained(tc::parts_kernel<D, T, false>, dim3(di.sms), dim3(tc::kThreads),
+                       fixed + tables, 1, true, stream, mk, mv, mq, mq1, tp);
   }
-  // Token splits of a sequence: a cluster of up to 8 blocks while the GPU has room for them.
-  const int nh = p.R > 8 ? 2 : 1;
-  const int hgs = (p.R + 8 * nh - 1) / (8 * nh);
-  const long long blocks = (long long)p.B * p.Hkv * hgs;
-  int ns = 1;
-  while (ns < 8 && blocks * ns * 2 <= 3ll * di.sms) ns *= 2;
-  const dim3 grid(ns, (unsigned)(p.Hkv * hgs), p.B);
-  // Without a prefix launch in front of it the own kernel has nothing to overlap with, and
-  // what it reads early would not be ordered behind earlier kernels.
-  return nh == 2 ? launch_chained(tc::own_kernel<D, 2, T>, grid, dim3(128), 0, ns, p.G > 0, stream, tp)
-                 : launch_chained(tc::own_kernel<D, 1, T>, grid, dim3(128), 0, ns, p.G > 0, stream, tp);
+  if (e != cudaSuccess) return e;
+  const long long out_rows = (long long)p.B * p.Hq;
+  constexpr int per = 256 / (D / 4);
+  return launch_chained(tc::join_kernel<D, T>, dim3((unsigned)((out_rows + per - 1) / per)),
+                        dim3(256), 0, 1, true, stream, tp);
 }
 
 cudaError_t launch_shared_prefix_decode(const void* q, const void* kp, const void* vp,
@@ -431,7 +466,7 @@ cudaError_t launch_shared_prefix_decode(const void* q, const void* kp, const voi
   p.scale_log2 = scale * 1.4426950408889634f;
   auto al = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
   if (!(flags & LLMC_DECODE_FORCE_GENERIC) && tc_shape(dtype, d, P, max_pages, B, Hq, Hkv, G) &&
-      al(q) && al(kp) && al(vp) && al(out)) {
+      al(q) && al(kp) && al(vp) && al(out) && scale > 0.f) {
     if (dtype == LLMC_BF16)
       return d == 128 ? launch_tc<128, __nv_bfloat16>(p, ws, dtype, err, stream)
                       : launch_tc<64, __nv_bfloat16>(p, ws, dtype, err, stream);

@@ -1,27 +1,36 @@
 // Shared-prefix decode attention on the tensor cores: bf16/fp16, head size 64 or 128.
 //
-// Two launches.  prefix_kernel computes the shared parts, own_kernel the sequences' own
-// parts and the join; own_kernel's attention needs nothing of prefix_kernel, so under
-// programmatic dependent launch it runs beside it and waits only before the join.
+// Two launches: parts_kernel leaves partial results, join_kernel joins them.
 //
-// prefix_kernel: rows = the query rows of a group that use one KV head (sequence, then
-// head), cut into tiles; a (group, KV head, row tile) is a unit, its tokens are cut into
-// chunks of 128, the chunks of all units are laid end to end, and CTA c of the persistent
-// grid takes chunks [c W / C, (c + 1) W / C) of the W.  The part of a unit inside a CTA's
-// range (a segment) leaves one partial in slot unit + c, which is unique because both
-// orders ascend.
-//   warps 0-3, 4-7   two softmax warpgroups ("streams"), one query row per thread;
-//   warp 8           TMA producer: pages of K and V into 128-byte-swizzled tiles;
+// parts_kernel works on units, of two kinds:
+//   shared: the query rows of a group that use one KV head (sequence, then head), cut into
+//           tiles, against the group's shared tokens;
+//   own:    the R query rows of a sequence that use one KV head against the tokens behind
+//           the shared ones.
+// The tokens of a unit are cut into chunks of 128.  The chunks of all units, shared ones
+// first, are laid end to end on a scale of costs (see Costs), and CTA c of the persistent
+// grid takes the chunks that begin in [c T / C, (c + 1) T / C) of the total T.  The part of
+// a unit inside a CTA's range is a segment.  CTAs on compute-bound shared units run beside
+// CTAs on memory-bound own units.
+//   warps 0-3, 4-7   two softmax warpgroups ("streams"), a query row per thread;
+//   warps 8, 10      TMA producers, 128-byte swizzled tiles: Q and K pages, V pages (a box
+//                    takes some 70 cycles to issue, and a page of 16 tokens is 4 KB of K);
+//   warp 11          the plan that join_kernel finds the partials by;
 //   warp 9           tcgen05 issuer: S = Q K^T (both in shared memory), O += P V (P in
 //                    TMEM over S's columns, V as an MN-major operand, so no transpose).
 // TMEM: S and O of both streams, 4 x 128 fp32 columns at head size 128 = all 512.
-// Row tiles of 128: chunks alternate between the streams (each with its own running
-// maximum, sum and O, joined through shared memory at the segment's end), so the softmax
-// of one chunk runs under the products of the next.  Row tiles of 256: a stream has 128 of
-// the rows and every chunk serves both, which halves the K/V traffic per row; used when
-// the work is long enough (see kLongChunks).
+//
+// Items: (chunk, row tile of 128) products, numbered through the CTA's range; item i belongs
+// to stream i & 1, so the softmax of one item runs under the products of the next, also
+// across segments.  The issuer runs S two items ahead of P V.  Segments with up to 128 rows
+// have one item per chunk: their chunks alternate between the streams, and each stream
+// leaves a partial of its own.  Segments with 256 rows ("wide") have two items per chunk,
+// which halves the K/V traffic per row; tiles are wide when the work is long enough that
+// the coarser split does no harm (kLongChunks).
+//
 // The running maximum is only raised when it would grow by more than 8 (log2): weights up
-// to 2^8 are harmless in 16 bits, and O is then rarely rescaled.
+// to 2^8 are harmless in 16 bits, and O is then rarely rescaled.  Rounded to 16 bits: the
+// weights P, as a tensor-core operand; the maximum, the sum, S and O are fp32.
 #pragma once
 
 #include "shared_prefix.cuh"
@@ -31,32 +40,87 @@ namespace prefix {
 namespace tc {
 
 constexpr int kChunk = 128;        // tokens of a chunk (MMA N of S, K of P V)
-constexpr int kThreads = 320;
-constexpr int kMaxGroups = 1024;   // group tables in shared memory: 24 bytes each
+constexpr int kRing = 8;            // segments the producer may be ahead
+constexpr int kThreads = 384;      // two softmax warpgroups, one for the producer and the issuer
 
-// Row tiles of 256 from this many 256-row chunks per CTA on.
+// Wide tiles from this many 256-row chunks per CTA on.
 constexpr int kLongChunks = 6;
-
-struct Plan {          // written by prefix_kernel's first CTA, read by own_kernel
-  int W, rt, pad[6];   // chunks in all, rows of a tile; then 4 ints per group:
-};                     // first chunk, first unit, chunks of a unit, rows
 
 struct TcParams {
   Params p;
-  int32_t* plan;
-  int rs_a, rs_b;      // rows of a slot with row tiles of 128 / 256
-  int ctas;            // grid of prefix_kernel
+  int4* plan;          // [B][Hkv], see below
+  int32_t* heads;      // tables_kernel's totals
+  int32_t* tables;     // the tables, where they are in global memory
+  float* own_o;        // partials of own units, beside p.part_o / part_lse of shared ones
+  float* own_lse;
+  int nb;              // sequences of a Q tile: nb * R <= 128 rows
+  int rs;              // rows of a shared slot
+  int ctas;            // grid of parts_kernel
 };
 
-__device__ __forceinline__ int cta_start(int c, int W, int C) {
-  return (int)((long long)c * W / C);
+// The plan: an int4 per (sequence, KV head), where join_kernel finds its partials:
+// {first shared slot, first own slot, shared slots | row << 16 | wide << 31, own slots}.
+
+// Partials of segment (unit u, CTA c): slots 2 (u + c) and 2 (u + c) + 1, unique because
+// units and ranges both ascend.  A slot is [D / 4][rows][4] fp32, so that the lanes of a
+// warp (rows) store 16-byte pieces side by side.
+
+// x / n for x >= 0, n > 0: the estimate is off by a few at most (24-bit mantissas).
+__device__ __forceinline__ int quot(int x, int n) {
+  int q = (int)(__int2float_rz(x) * __frcp_rn((float)n));
+  int r = x - q * n;
+  while (r < 0) {
+    --q;
+    r += n;
+  }
+  while (r >= n) {
+    ++q;
+    r -= n;
+  }
+  return q;
 }
-__device__ __forceinline__ int cta_owner(int u, int W, int C) {
-  int c = (int)((long long)u * C / W);
-  while (c + 1 < C && cta_start(c + 1, W, C) <= u) ++c;
-  while (c > 0 && cta_start(c, W, C) > u) --c;
-  return c;
-}
+
+// What the chunks cost, in units of some 1100 cycles: a chunk of 128 rows at most 3 (K and V
+// of 64 KB at a fair share of the bandwidth are 2700 cycles), a chunk of a wide tile 4, and a
+// unit of own tokens 2 more, for the turn-over of a stream (measured: own units of n chunks
+// 2500 + 3400 n cycles, wide chunks 4400).  With few chunks for the CTAs every chunk is 1.
+struct Costs {
+  int shared, own, unit;
+  __device__ __forceinline__ void set(int chunks, bool wide, int ctas) {
+    const bool few = chunks < 2 * ctas;   // otherwise every CTA's share exceeds own + unit
+    shared = few ? 1 : wide ? 4 : 3;
+    own = few ? 1 : 3;
+    unit = few ? 0 : 2;
+  }
+  // where chunk j of an own unit begins, and the first chunk that begins at x or later
+  __device__ __forceinline__ int at(int j) const { return j ? unit + j * own : 0; }
+  __device__ __forceinline__ int chunk_from(int x) const {
+    return x <= 0 ? 0 : max(1, quot(max(0, x - unit) + own - 1, own));
+  }
+};
+
+// How the total cost is dealt to C CTAs.
+struct Split {
+  int C, total, q, r;
+  __device__ __forceinline__ void set(int total_, int ctas) {
+    total = total_;
+    // With fewer chunks than CTAs the first ones have one each: no CTA between a unit's first
+    // and last is without a part of it.
+    C = min(ctas, total);
+    q = C ? quot(total, C) : 0;
+    r = total - q * C;
+  }
+  __device__ __forceinline__ int start(int c) const {   // floor(c total / C), c <= C
+    return c * q + quot(c * r, C);
+  }
+  __device__ __forceinline__ int owner(int x) const {   // the last c with start(c) <= x
+    const long long ec = (long long)(x + 1) * C;        // start(c) <= x  <=>  c total < (x + 1) C
+    int c = min(C - 1, (int)((float)x * (float)C * __frcp_rn((float)total)));
+    while (c + 1 < C && (long long)(c + 1) * total < ec) ++c;
+    while (c > 0 && (long long)c * total >= ec) --c;
+    return c;
+  }
+};
 
 // ---- tcgen05 -------------------------------------------------------------------
 __device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
@@ -64,11 +128,13 @@ __device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) |
          (2ull << 61);
 }
-__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr) {
-  // 128-byte swizzle, 64 contiguous N elements per row (a token), 8-token groups 1024 bytes
-  // apart (stride offset), the next 64 N elements kChunk rows further (leading offset).
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(kChunk * 128 / 16) << 16) |
-         (64ull << 32) | (1ull << 46) | (2ull << 61);
+__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr, int box) {
+  // 128-byte swizzle, 64 contiguous N elements per row (a token), laid out [box][half][rows]:
+  // the other 64 N elements are a box's rows further (leading offset), the next 8 tokens
+  // follow (stride offset) unless a box holds only 8.
+  const uint32_t lead = (uint32_t)box * 128, stride = box == 8 ? 2 * lead : 1024u;
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) |
+         ((uint64_t)(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                        uint32_t acc) {
@@ -117,6 +183,16 @@ __device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
       : "r"(addr)
       : "memory");
 }
+__device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
 __device__ __forceinline__ void st32(uint32_t addr, const uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -146,7 +222,26 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void bar_softmax() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// Two fp32 operations at once (register pairs).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 template <int D>
 struct Smem {
@@ -154,68 +249,330 @@ struct Smem {
   static constexpr int kHalves = D / 64;
   static constexpr int kStages = D == 128 ? 2 : 4;
   static constexpr int kOperand = kHalves * kTile;        // a Q tile, a K or V chunk
-  static constexpr int kQ = 0;                            // 2 Q tiles; the join's exchange
+  static constexpr int kQ = 0;                            // 2 Q tiles
   static constexpr int kK = 2 * kOperand;
   static constexpr int kV = kK + kStages * kOperand;
   static constexpr int kBars = kV + kStages * kOperand;
-  static constexpr int kNumBars = 4 * kStages + 7;
+  static constexpr int kNumBars = 4 * kStages + 10 + 2 * kRing;
   static constexpr int kMisc = kBars + 8 * kNumBars;      // tmem slot, abort flag, totals
-  static constexpr int kMl = kMisc + 24;                  // [2][128] (max, sum)
-  static constexpr int kGroups = kMl + 2 * 128 * 8;
-  static size_t bytes(int G) { return 1024 + kGroups + sizeof(int) * (6 * (size_t)G + 1); }
+  static constexpr int kSegs = kMisc + 32;                // [kRing] segments
+  static constexpr int kTables = kSegs + 48 * kRing;
 };
 
-// A segment: the part of a unit in this CTA's range.
-struct Segment {
-  int g, hk, tile, unit, ch0, n, s, leader, lo, rows;   // rows: valid rows of the tile
-};
-
-// Group tables in shared memory.
-struct Groups {
-  int* start;    // [G] first chunk of the group
-  int* unit;     // [G] first unit
+// Tables of the groups and sequences, in shared or global memory.
+struct Tables {
+  int* lo;       // [G + 1] first sequence
   int* s;        // [G] shared tokens
   int* leader;   // [G] sequence whose table row is read
-  int* lo;       // [G + 1] first sequence
   int* rows;     // [G] query rows per KV head
+  int* start;    // [G] where its units begin on the scale of costs
+  int* unit;     // [G] first unit
+  int* len;      // [B] length
+  int* gid;      // [B] group or -1
+  int* own;      // [B] where its own units begin, behind all shared ones
+  __host__ __device__ static size_t ints(int G, int B) { return 6 * (size_t)G + 1 + 3 * (size_t)B; }
+  __device__ __forceinline__ void place(int* base, int G, int B) {
+    lo = base; s = lo + G + 1; leader = s + G; rows = leader + G; start = rows + G;
+    unit = start + G; len = unit + G; gid = len + B; own = gid + B;
+  }
 };
 
-__device__ __forceinline__ bool next_segment(const TcParams& tp, const Groups& gr, int rt, int& c,
-                                             int c1, int& g, Segment& sg) {
-  if (c >= c1) return false;
-  const int G = tp.p.G, Hkv = tp.p.Hkv;
-  int nch, tiles;
-  while (true) {   // the group that holds chunk c
-    nch = (gr.s[g] + kChunk - 1) / kChunk;
-    tiles = (gr.rows[g] + rt - 1) / rt;
-    if (c < gr.start[g] + nch * tiles * Hkv || g + 1 >= G) break;
-    ++g;
-  }
-  const int x = c - gr.start[g], ul = x / nch;
-  sg.g = g;
-  sg.hk = ul / tiles;
-  sg.tile = ul - sg.hk * tiles;
-  sg.unit = gr.unit[g] + ul;
-  sg.ch0 = x - ul * nch;
-  sg.n = min(nch - sg.ch0, c1 - c);
-  sg.s = gr.s[g];
-  sg.leader = gr.leader[g];
-  sg.lo = gr.lo[g];
-  sg.rows = min(rt, gr.rows[g] - sg.tile * rt);
-  c += sg.n;
-  return true;
+// First token of a sequence's chunk grid: whole boxes of a page.
+__device__ __forceinline__ int own_base(const Params& p, int s) {
+  return s & ~(min(p.P, kChunk) - 1);   // a power of two
+}
+__device__ __forceinline__ int own_chunks(const Params& p, int s, int len) {
+  return len > s ? (len - own_base(p, s) + kChunk - 1) / kChunk : 0;
 }
 
-template <int D, typename T>
+// Builds the tables with threads tid = 0 .. nt - 1 (whole warps; barrier 1).  totals: cost of
+// the shared units, of all, rows of a tile, chunks in all.  Inlined, so that tables in shared memory are
+// accessed as such.
+__device__ __forceinline__ void bar1(int nt) { asm volatile("bar.sync 1, %0;" ::"r"(nt) : "memory"); }
+__device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t, int* totals,
+                                             int ctas, int tid, int nt) {
+  const Params& p = tp.p;
+  const int lane = tid & 31;
+  // The last warps fetch the groups, the others the lengths: one round trip for both.
+  for (int g = nt - 1 - tid; g <= p.G; g += nt) {
+    t.lo[g] = p.G ? p.starts[g] : 0;
+    if (g < p.G) {
+      t.s[g] = 0x7fffffff;
+      t.leader[g] = 0x7fffffff;
+      t.unit[g] = p.shared[g];
+    }
+  }
+  for (int b = tid; b < p.B; b += nt) t.len[b] = seq_len(p, b, true);
+  bar1(nt);
+  for (int b = tid; b < p.B; b += nt) {
+    const int n = t.len[b];
+    int gid = -1;
+    if (p.G) {
+      int a = 0, z = p.G;     // the last group that starts at or before b
+      while (z - a > 1) {
+        const int mid = (a + z) >> 1;
+        if (t.lo[mid] <= b) a = mid; else z = mid;
+      }
+      const int lo = t.lo[a], hi = t.lo[a + 1];
+      if (n > 0 && lo >= 0 && hi <= p.B && b >= lo && b < hi && b - lo < p.max_group) {
+        gid = a;
+        atomicMin(&t.s[a], n);
+        atomicMin(&t.leader[a], b);
+      }
+    }
+    t.gid[b] = gid;
+  }
+  bar1(nt);
+  if (tid < 32) {   // the groups, with prefix sums for narrow and for wide tiles
+    // One bad range and nothing is shared: overlapping groups would pass the workspace.
+    int bad = 0;
+    for (int g = lane; g < p.G; g += 32)
+      bad |= t.lo[g] < 0 || t.lo[g + 1] < t.lo[g] || t.lo[g + 1] > p.B;
+    bad = __any_sync(0xffffffffu, bad);
+    if (bad && lane == 0) atomicOr(p.status, kStatusBadGroup);
+    const int narrow = tp.nb * p.R;
+    const int per = (p.G + 31) >> 5, g0 = min(lane * per, p.G), g1 = min(g0 + per, p.G);
+    int w0 = 0, w1 = 0, u0 = 0, u1 = 0, most = 0;
+    for (int g = g0; g < g1; ++g) {   // a lane's groups with either tile
+      int n = 0, rows = 0;
+      if (!bad && t.leader[g] != 0x7fffffff) {
+        n = max(0, min(t.unit[g], t.s[g]));
+        rows = min(t.lo[g + 1] - t.lo[g], p.max_group) * p.R;
+      }
+      t.s[g] = n;
+      t.rows[g] = rows;
+      if (n) {
+        const int ch = (n + kChunk - 1) / kChunk, ta = quot(rows + narrow - 1, narrow);
+        u0 += ta * p.Hkv;
+        u1 += (ta + 1) / 2 * p.Hkv;
+        w0 += ch * ta * p.Hkv;
+        w1 += ch * ((ta + 1) / 2) * p.Hkv;
+        most = max(most, rows);
+      }
+    }
+    const bool wide = __reduce_max_sync(0xffffffffu, most) > narrow &&
+                      __reduce_add_sync(0xffffffffu, w1) >= kLongChunks * ctas;
+    const int rt = wide ? 2 * narrow : narrow;
+    // own chunks and units of this lane's sequences
+    const int bper = (p.B + 31) >> 5, b0 = min(lane * bper, p.B), b1 = min(b0 + bper, p.B);
+    __syncwarp();
+    int oc = 0, ou = 0;
+    for (int b = b0; b < b1; ++b) {
+      int gid = t.gid[b];
+      if (gid >= 0 && t.s[gid] == 0) t.gid[b] = gid = -1;
+      const int n = own_chunks(p, gid >= 0 ? t.s[gid] : 0, t.len[b]);
+      oc += n * p.Hkv;
+      ou += n ? p.Hkv : 0;
+    }
+    const int chunks = __reduce_add_sync(0xffffffffu, (wide ? w1 : w0) + oc);
+    Costs cost;
+    cost.set(chunks, wide, ctas);
+    const int wl = (wide ? w1 : w0) * cost.shared, ul = wide ? u1 : u0;
+    const int xl = oc * cost.own + ou * cost.unit;
+    int cs = wl, us = ul, xs = xl;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, cs, o), b = __shfl_up_sync(0xffffffffu, us, o);
+      const int d = __shfl_up_sync(0xffffffffu, xs, o);
+      if (lane >= o) {
+        cs += a;
+        us += b;
+        xs += d;
+      }
+    }
+    if (lane == 31) {
+      totals[0] = cs;
+      totals[1] = cs + xs;
+      totals[2] = rt;
+      totals[3] = chunks;
+    }
+    cs -= wl;
+    us -= ul;
+    xs -= xl;
+    for (int g = g0; g < g1; ++g) {
+      t.start[g] = cs;
+      t.unit[g] = us;
+      if (t.s[g]) {
+        const int ta = quot(t.rows[g] + rt - 1, rt) * p.Hkv;
+        us += ta;
+        cs += ta * ((t.s[g] + kChunk - 1) / kChunk) * cost.shared;
+      }
+    }
+    for (int b = b0; b < b1; ++b) {
+      t.own[b] = xs;
+      const int gid = t.gid[b], n = own_chunks(p, gid >= 0 ? t.s[gid] : 0, t.len[b]);
+      xs += n ? (n * cost.own + cost.unit) * p.Hkv : 0;
+    }
+  }
+  bar1(nt);
+}
+
+// The plan's entries first, first + step, ...
+__device__ __forceinline__ void write_plan(const TcParams& tp, const Tables& t, const int* totals,
+                                           int ctas, int first, int step) {
+  const Params& p = tp.p;
+  const int narrow = tp.nb * p.R, rt = totals[2];
+  Split split;
+  split.set(totals[1], ctas);
+  Costs cost;
+  cost.set(totals[3], rt > narrow, ctas);
+  for (int e = first; e < p.B * p.Hkv; e += step) {
+    const int b = quot(e, p.Hkv), hk = e - b * p.Hkv, g = t.gid[b];
+    int4 v = make_int4(0, 0, 0, 0);
+    int s = 0;
+    if (g >= 0) {
+      s = t.s[g];
+      const int nch = (s + kChunk - 1) / kChunk, tiles = quot(t.rows[g] + rt - 1, rt);
+      const int rr = (b - t.lo[g]) * p.R, tile = quot(rr, rt), u = hk * tiles + tile;
+      const bool wide = min(rt, t.rows[g] - tile * rt) > narrow;
+      const int q = wide && rr - tile * rt >= narrow ? 1 : 0;
+      const int x = t.start[g] + u * nch * cost.shared, a = split.owner(x);
+      const int segs = split.owner(x + (nch - 1) * cost.shared) - a + 1;
+      v.x = 2 * (t.unit[g] + u + a) + q;
+      v.z = (wide ? segs : 2 * segs) | (rr - tile * rt - q * narrow) << 16 |
+            (wide ? (int)0x80000000 : 0);
+    }
+    const int nch = own_chunks(p, s, t.len[b]);
+    if (nch) {
+      const int x = totals[0] + t.own[b] + hk * (nch * cost.own + cost.unit), a = split.owner(x);
+      v.y = 2 * (e + a);
+      v.w = 2 * (split.owner(x + cost.at(nch - 1)) - a + 1);
+    }
+    tp.plan[e] = v;
+  }
+}
+
+// For batches whose tables do not fit shared memory: one block builds them in global memory.
+__global__ void __launch_bounds__(1024) tables_kernel(const __grid_constant__ TcParams tp) {
+  __shared__ int totals[4];
+  pdl_wait();
+  Tables t;
+  t.place(tp.tables, tp.p.G, tp.p.B);
+  build_tables(tp, t, totals, tp.ctas, threadIdx.x, blockDim.x);
+  __syncthreads();
+  if (threadIdx.x < 4) tp.heads[threadIdx.x] = totals[threadIdx.x];
+  pdl_launch_dependents();
+}
+
+// A segment: the part of a unit in a CTA's range.  The producer walks them and publishes
+// each in a ring in shared memory; n = 0 ends the list.
+struct __align__(16) Segment {
+  int n;         // chunks
+  int wide;
+  int t0;        // first token of the segment's first chunk
+  int hi;        // end of the unit's tokens
+  int lo;        // their start
+  int rows, slot, own;   // slot: first of its two
+  int hk, b_table, b_q, pad;
+};
+static_assert(sizeof(Segment) == 48, "ring entries of 48 bytes");
+
+// Walks the segments of the chunks that begin in [x, x1).
+struct Walker {
+  int x, x1, g, b, X0, rt;   // X0: cost of the shared units
+  Costs cost;
+
+  // The last of n ascending entries that is <= x (0 if none), by a whole warp.
+  static __device__ __forceinline__ int find(const int* a, int n, int x) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0;
+    while (n > 1) {
+      const int step = (n + 31) >> 5, i = lane * step;
+      const int k = __popc(__ballot_sync(0xffffffffu, i < n && a[lo + i] <= x));
+      const int at = k ? (k - 1) * step : 0;
+      lo += at;
+      n = min(step, n - at);
+    }
+    return lo;
+  }
+  __device__ __forceinline__ void init(const TcParams& tp, const Tables& t, const int* totals) {
+    const Params& p = tp.p;
+    X0 = totals[0];
+    rt = totals[2];
+    cost.set(totals[3], rt > tp.nb * p.R, gridDim.x);
+    Split split;
+    split.set(totals[1], gridDim.x);
+    const bool idle = (int)blockIdx.x >= split.C;
+    x = idle ? 0 : split.start(blockIdx.x);
+    x1 = idle ? 0 : split.start(blockIdx.x + 1);
+    g = x < X0 ? find(t.start, p.G, x) : 0;
+    b = x1 > X0 ? find(t.own, p.B, max(0, x - X0)) : 0;
+  }
+  __device__ __forceinline__ bool next(const TcParams& tp, const Tables& t, Segment& sg) {
+    const Params& p = tp.p;
+    while (x < x1) {
+      int j0, j1;
+      if (x < X0) {
+        int nch, tiles, size;
+        while (true) {   // the group that holds x
+          nch = (t.s[g] + kChunk - 1) / kChunk;
+          tiles = quot(t.rows[g] + rt - 1, rt);
+          size = nch * cost.shared;
+          if (x < t.start[g] + size * tiles * p.Hkv || g + 1 >= p.G) break;
+          ++g;
+        }
+        const int y = x - t.start[g], ul = quot(y, size), base = x - (y - ul * size);
+        j0 = quot(x - base + cost.shared - 1, cost.shared);
+        j1 = min(nch, quot(x1 - base + cost.shared - 1, cost.shared));
+        x = min(x1, base + size);
+        sg.hk = quot(ul, tiles);
+        const int tile = ul - sg.hk * tiles;
+        sg.own = 0;
+        sg.b_table = t.leader[g];
+        sg.b_q = t.lo[g] + tile * (rt > tp.nb * p.R ? 2 * tp.nb : tp.nb);
+        sg.rows = min(rt, t.rows[g] - tile * rt);
+        sg.wide = sg.rows > tp.nb * p.R;
+        sg.t0 = j0 * kChunk;
+        sg.lo = 0;
+        sg.hi = t.s[g];
+        sg.slot = 2 * (t.unit[g] + ul + (int)blockIdx.x);
+      } else {
+        int nch, s, size;
+        while (true) {   // the sequence that holds x
+          s = t.gid[b] >= 0 ? t.s[t.gid[b]] : 0;
+          nch = own_chunks(p, s, t.len[b]);
+          size = nch ? nch * cost.own + cost.unit : 0;
+          if (x - X0 < t.own[b] + size * p.Hkv || b + 1 >= p.B) break;
+          ++b;
+        }
+        const int y = x - X0 - t.own[b], hk = quot(y, size), base = x - (y - hk * size);
+        j0 = cost.chunk_from(x - base);
+        j1 = min(nch, cost.chunk_from(x1 - base));
+        x = min(x1, base + size);
+        sg.own = 1;
+        sg.hk = hk;
+        sg.b_table = b;
+        sg.b_q = b;
+        sg.rows = p.R;
+        sg.wide = 0;
+        sg.t0 = own_base(p, s) + j0 * kChunk;
+        sg.lo = s;
+        sg.hi = t.len[b];
+        sg.slot = 2 * (b * p.Hkv + hk + (int)blockIdx.x);
+      }
+      sg.n = j1 - j0;
+      if (sg.n > 0) return true;   // none: x was in the last chunk of its unit
+    }
+    return false;
+  }
+};
+
+// The issuer's place in the items of the CTA.
+struct Cursor {
+  int n, wide, t0, hi;             // of the segment; n = 0: past the last
+  int j, sub, item, k, qc, seg;    // chunk and row tile in the segment; running counters
+};
+
+template <int D, typename T, bool kGlobalTables>
 __global__ void __launch_bounds__(kThreads, 1)
-prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-              const __grid_constant__ TcParams tp) {
+parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+             const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_q1,
+             const __grid_constant__ TcParams tp) {
   using S = Smem<D>;
   constexpr int NS = S::kStages;
-  constexpr uint32_t FMT = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
-  // fp32 accumulate, M = 128; S: N = 128, both K-major; P V: N = D, V MN-major (bit 16).
-  constexpr uint32_t ID_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((uint32_t)(kChunk >> 3) << 17) |
-                            (8u << 24);
+  constexpr uint32_t FMT = __is_same(T, __nv_bfloat16) ? 1u : 0u;
+  // fp32 accumulate, M = 128; S: both K-major, N = tokens; P V: N = D, V MN-major (bit 16).
+  constexpr uint32_t ID_S = (1u << 4) | (FMT << 7) | (FMT << 10) | (8u << 24);
   constexpr uint32_t ID_O = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) |
                             ((uint32_t)(D >> 3) << 17) | (8u << 24);
   const Params& p = tp.p;
@@ -225,18 +582,12 @@ prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
   const uint32_t bars = sb + S::kBars;
   const uint32_t kfull = bars, kempty = kfull + 8 * NS, vfull = kempty + 8 * NS,
                  vempty = vfull + 8 * NS, sfull = vempty + 8 * NS, pready = sfull + 16,
-                 ofull = pready + 16, qready = ofull + 16;
+                 ofull = pready + 16, qfull = ofull + 16, qempty = qfull + 16,
+                 gfull = qempty + 16, gempty = gfull + 8 * kRing;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + S::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + S::kMisc + 4);
-  int* total = reinterpret_cast<int*>(smem + S::kMisc + 8);   // W, rt
-  float2* ml = reinterpret_cast<float2*>(smem + S::kMl);
-  Groups gr;
-  gr.start = reinterpret_cast<int*>(smem + S::kGroups);
-  gr.unit = gr.start + p.G;
-  gr.s = gr.unit + p.G;
-  gr.leader = gr.s + p.G;
-  gr.rows = gr.leader + p.G;
-  gr.lo = gr.rows + p.G;
+  int* totals = reinterpret_cast<int*>(smem + S::kMisc + 8);
+  const Segment* segs = reinterpret_cast<const Segment*>(smem + S::kSegs);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
@@ -250,12 +601,19 @@ prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       mbar_init(sfull + 8 * i, 1);
       mbar_init(pready + 8 * i, 128);
       mbar_init(ofull + 8 * i, 1);
+      mbar_init(qfull + 8 * i, 1);
+      mbar_init(qempty + 8 * i, 1);
     }
-    mbar_init(qready, 256);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(gfull + 8 * i, 1);
+      mbar_init(gempty + 8 * i, 10);   // the issuer, the V producer, eight softmax warps
+    }
     *abort_flag = 0;
     fence_mbarrier_init();
     prefetch_tensormap(&map_k);
     prefetch_tensormap(&map_v);
+    prefetch_tensormap(&map_q);
+    prefetch_tensormap(&map_q1);
   }
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -264,157 +622,108 @@ prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  pdl_wait();               // lengths, queries and pages come from earlier kernels
-  pdl_launch_dependents();  // after the wait: what own_kernel reads early is then final
-
-  // ---- the groups and this CTA's range ----
-  for (int g = tid; g <= p.G; g += kThreads) {
-    gr.lo[g] = p.starts[g];
-    if (g < p.G) {
-      gr.s[g] = 0x7fffffff;
-      gr.leader[g] = 0x7fffffff;
-    }
-  }
-  __syncthreads();
-  for (int b = tid; b < p.B; b += kThreads) {
-    const int n = seq_len(p, b, false);
-    if (n <= 0) continue;
-    int a = 0, z = p.G;     // the last group that starts at or before b
-    while (z - a > 1) {
-      const int mid = (a + z) >> 1;
-      if (gr.lo[mid] <= b) a = mid; else z = mid;
-    }
-    const int lo = gr.lo[a], hi = gr.lo[a + 1];
-    if (lo >= 0 && hi <= p.B && b >= lo && b < hi && b - lo < p.max_group) {
-      atomicMin(&gr.s[a], n);
-      atomicMin(&gr.leader[a], b);
-    }
-  }
-  // One bad range and nothing is shared: overlapping groups would pass the workspace.
-  int bad = 0;
-  for (int g = tid; g < p.G; g += kThreads)
-    bad |= gr.lo[g] < 0 || gr.lo[g + 1] < gr.lo[g] || gr.lo[g + 1] > p.B;
-  bad = __syncthreads_or(bad);
-  if (bad && tid == 0) atomicOr(p.status, kStatusBadGroup);
-  for (int g = tid; g < p.G; g += kThreads) {
-    const bool any = !bad && gr.leader[g] != 0x7fffffff;
-    gr.s[g] = any ? max(0, min(p.shared[g], gr.s[g])) : 0;
-    gr.rows[g] = any ? min(gr.lo[g + 1] - gr.lo[g], p.max_group) * p.R : 0;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    int rt = 128, w = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-      // pass 0: would row tiles of 256 give every CTA kLongChunks?  pass 1: the prefix sums
-      rt = pass == 0 ? 256 : rt;
-      int u = 0, most = 0;
-      w = 0;
-      for (int g0 = 0; g0 < p.G; g0 += 32) {
-        const int g = g0 + lane;
-        int units = 0, chunks = 0;
-        if (g < p.G && gr.s[g] > 0) {
-          units = (gr.rows[g] + rt - 1) / rt * p.Hkv;
-          chunks = units * ((gr.s[g] + kChunk - 1) / kChunk);
-          most = max(most, gr.rows[g]);
-        }
-        int cs = chunks, us = units;
-        for (int o = 1; o < 32; o <<= 1) {
-          const int a = __shfl_up_sync(0xffffffffu, cs, o), b = __shfl_up_sync(0xffffffffu, us, o);
-          if (lane >= o) {
-            cs += a;
-            us += b;
-          }
-        }
-        if (pass == 1 && g < p.G) {
-          gr.start[g] = w + cs - chunks;
-          gr.unit[g] = u + us - units;
-        }
-        w += __shfl_sync(0xffffffffu, cs, 31);
-        u += __shfl_sync(0xffffffffu, us, 31);
-      }
-      if (pass == 0) {
-        for (int o = 16; o; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-        rt = most > 128 && w >= kLongChunks * (int)gridDim.x ? 256 : 128;
-      }
-    }
-    if (lane == 0) {
-      total[0] = w;
-      total[1] = rt;
-    }
-  }
+  pdl_launch_dependents();
   fence_before();
   __syncthreads();
   fence_after();
-  const int W = total[0], rt = total[1];
   const uint32_t tmem = *tmem_slot;
-  // With fewer chunks than CTAs the first W have one each: no CTA between a unit's first and
-  // last is without a part of it.
-  const int C = min((int)gridDim.x, W);
-  const bool idle = (int)blockIdx.x >= C;
-  const int c0 = idle ? 0 : cta_start(blockIdx.x, W, C);
-  const int c1 = idle ? 0 : cta_start(blockIdx.x + 1, W, C);
-  if (blockIdx.x == 0) {   // what own_kernel needs to find the partials
-    if (tid == 0) {
-      tp.plan[0] = W;
-      tp.plan[1] = rt;
-    }
-    for (int g = tid; g < p.G; g += kThreads) {
-      int4 v = make_int4(gr.start[g], gr.unit[g], (gr.s[g] + kChunk - 1) / kChunk, gr.rows[g]);
-      reinterpret_cast<int4*>(tp.plan + 8)[g] = v;
-    }
-  }
-  const bool wide = rt == 256;   // both streams serve every chunk
-  int g = 0;
-  if (c0 < c1) {                 // the first group of the range
-    int a = 0, z = p.G;
-    while (z - a > 1) {
-      const int mid = (a + z) >> 1;
-      if (gr.start[mid] <= c0) a = mid; else z = mid;
-    }
-    g = a;
-  }
-  Segment sg;
-  int c = c0;
+  Tables t;
+  if (kGlobalTables)
+    t.place(tp.tables, p.G, p.B);
+  else
+    t.place(reinterpret_cast<int*>(smem + S::kTables), p.G, p.B);
 
-  if (warp == 8) {
-    // ---- TMA producer: lane i brings page i of the chunk ----
-    const int box = min(p.P, kChunk), ppc = kChunk / box;   // box rows, boxes per chunk
-    int cnt = 0;
-    while (next_segment(tp, gr, rt, c, c1, g, sg)) {
-      const int32_t* row = p.block_table + (long long)sg.leader * p.max_pages;
-      auto page_at = [&](int ch) -> int {
-        const int tok = (sg.ch0 + ch) * kChunk + lane * box;
-        return ch < sg.n && lane < ppc && tok < sg.s ? row[tok / p.P] : 0;
+  // Registers: 12 warps, three per scheduler, start with 168 each (504 of a scheduler's 512 a
+  // lane); the softmax warps take what the others give up.
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  pdl_wait();               // lengths, queries and pages come from earlier kernels
+  if (kGlobalTables) {      // built by tables_kernel
+    if (tid < 256 + 4) totals[tid - 256] = tp.heads[tid - 256];
+    bar1(128);
+  } else {
+    build_tables(tp, t, totals, gridDim.x, tid - 256, 128);
+  }
+  if (warp == 8 || warp == 10) {
+    // ---- TMA producers: lane i brings page (or part of a page) i of the chunk.  Warp 8
+    // walks the segments, publishes them and brings Q and K, warp 10 brings V. ----
+    const bool isv = warp == 10;
+    const int box = min(p.P, kChunk), bsh = 31 - __clz(box);   // box rows: a power of two
+    const int ppc = kChunk >> bsh;                             // boxes per chunk
+    const uint32_t tile0 = sb + (isv ? S::kV : S::kK);
+    const uint32_t fulls = isv ? vfull : kfull, empties = isv ? vempty : kempty;
+    int k = 0, qc = 0;
+    Walker w0;
+    if (!isv) w0.init(tp, t, totals);
+    for (int ns = 0;; ++ns) {
+      Segment sg;
+      const int slot = ns % kRing;
+      Segment* entry = reinterpret_cast<Segment*>(smem + S::kSegs) + slot;
+      if (!isv) {
+        if (!w0.next(tp, t, sg)) sg.n = 0;
+        mbar_wait_bounded(gempty + 8 * slot, ((ns / kRing) & 1) ^ 1, abort_flag, p.status);
+        if (lane == 0) {
+          *entry = sg;
+          mbar_arrive(gfull + 8 * slot);
+        }
+        __syncwarp();
+      } else {
+        mbar_wait_bounded(gfull + 8 * slot, (ns / kRing) & 1, abort_flag, p.status);
+        sg = *entry;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(gempty + 8 * slot);
+      }
+      if (__any_sync(0xffffffffu, sg.n == 0 || *abort_flag != 0)) break;
+      const int32_t* row = p.block_table + (long long)sg.b_table * p.max_pages;
+      auto page_at = [&](int j) -> int {
+        const int tok = sg.t0 + j * kChunk + (lane << bsh);
+        if (j >= sg.n || lane >= ppc || tok >= sg.hi) return 0;
+        return row[p.P <= kChunk ? tok >> bsh : quot(tok, p.P)];
       };
       int next = page_at(0);
-      for (int j = 0; j < sg.n; ++j, ++cnt) {
-        const int st = cnt % NS;
-        const uint32_t par = ((cnt / NS) & 1) ^ 1;
-        const int t0 = (sg.ch0 + j) * kChunk;
-        const int boxes = min(ppc, (sg.s - t0 + box - 1) / box);
+      if (!isv) {
+        for (int q = 0; q <= sg.wide; ++q, ++qc) {
+          const int qb = qc & 1;
+          mbar_wait_bounded(qempty + 8 * qb, ((qc >> 1) & 1) ^ 1, abort_flag, p.status);
+          if (lane == 0 && !*abort_flag) {
+            mbar_arrive_expect_tx(qfull + 8 * qb, (uint32_t)((sg.own ? 1 : tp.nb) * p.R * D * 2));
+#pragma unroll
+            for (int h = 0; h < S::kHalves; ++h)
+              tma_load_3d(sb + S::kQ + qb * S::kOperand + h * S::kTile, sg.own ? &map_q1 : &map_q,
+                          h * 64, sg.hk * p.R, sg.b_q + q * tp.nb, qfull + 8 * qb);
+          }
+          __syncwarp();
+        }
+      }
+      for (int j = 0; j < sg.n; ++j, ++k) {
+        const int st = k % NS;
+        const int t0 = sg.t0 + j * kChunk;
+        const int boxes = min(ppc, (sg.hi - t0 + box - 1) >> bsh);
         int page = next;
         next = page_at(j + 1);
         if (page < 0 || page >= p.num_pages) {
           atomicOr(p.status, kStatusBadPage);
           page = 0;
         }
-        const int y = (int)(((long long)page * p.Hkv + sg.hk) * p.P + (t0 + lane * box) % p.P);
-        const uint32_t bytes = (uint32_t)(boxes * box * D * 2);
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          const uint32_t full = (kv ? vfull : kfull) + 8 * st, empty = (kv ? vempty : kempty) + 8 * st;
-          mbar_wait_bounded(empty, par, abort_flag, p.status);
-          const bool go = !*abort_flag;
-          if (lane == 0 && go) mbar_arrive_expect_tx(full, bytes);
-          __syncwarp();
-          if (go && lane < boxes) {
-            const uint32_t dst = sb + (kv ? S::kV : S::kK) + st * S::kOperand + lane * box * 128;
+        int in_page = 0;      // a page of more than a chunk: where in it
+        if (p.P > kChunk) in_page = t0 - quot(t0, p.P) * p.P;
+        const int y = (page * p.Hkv + sg.hk) * p.P + in_page;   // pool rows: below 2^31
+        mbar_wait_bounded(empties + 8 * st, ((k / NS) & 1) ^ 1, abort_flag, p.status);
+        const bool go = !*abort_flag;
+        const uint32_t full = fulls + 8 * st;
+        if (lane == 0 && go) mbar_arrive_expect_tx(full, (uint32_t)(boxes * box * D * 2));
+        __syncwarp();
+        if (go && lane < boxes) {
+          const uint32_t dst = tile0 + st * S::kOperand;
+          if (isv) {       // [box][half][rows]: both halves in one copy
+            tma_load_3d(dst + lane * (box * 128 * S::kHalves), &map_v, 0, y, 0, full);
+          } else {         // [half][rows of all boxes]: 8-row groups evenly spaced
 #pragma unroll
             for (int h = 0; h < S::kHalves; ++h)
-              tma_load_2d(dst + h * S::kTile, kv ? &map_v : &map_k, h * 64, y, full);
+              tma_load_2d(dst + lane * box * 128 + h * S::kTile, &map_k, h * 64, y, full);
           }
-          __syncwarp();
         }
+        __syncwarp();
       }
     }
     if (*abort_flag) {   // let the copies in flight land before the block goes
@@ -422,260 +731,279 @@ prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
       while (globaltimer_ns() - t0 < 2000000ull) {
       }
     }
+  } else if (warp == 11) {
+    write_plan(tp, t, totals, gridDim.x, blockIdx.x * 32 + lane, gridDim.x * 32);
   } else if (warp == 9) {
     // ---- tcgen05 issuer ----
+    asm volatile("bar.sync 2, 288;" ::: "memory");   // the softmax warps' rehearsal is over
     if (lane == 0) {
-      int cnt = 0, nseg = 0, items_s[2] = {0, 0};
-      while (next_segment(tp, gr, rt, c, c1, g, sg)) {
-        const int items = wide ? 2 * sg.n : sg.n;
-        mbar_wait_bounded(qready, nseg & 1, abort_flag, p.status);
-        fence_after();
-        auto issue_s = [&](int i) {   // S of item i: stream i & 1
-          const int s = i & 1, ch = wide ? i >> 1 : i, k = cnt + ch, st = k % NS;
-          if (!wide || s == 0) mbar_wait_bounded(kfull + 8 * st, (k / NS) & 1, abort_flag, p.status);
-          fence_after();
-          const uint32_t a = sb + S::kQ + (wide ? s : 0) * S::kOperand;
-          const uint32_t b = sb + S::kK + st * S::kOperand;
-#pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk / 4) * S::kTile + (kk % 4) * 32;
-            mma_ss(tmem + s * 128, desc_kmajor(a + off), desc_kmajor(b + off), ID_S, kk > 0);
-          }
-          commit(sfull + 8 * s);
-          if (!wide || s == 1) commit(kempty + 8 * st);
-        };
-        issue_s(0);
-        if (items > 1) issue_s(1);
-        for (int i = 0; i < items; ++i) {
-          const int s = i & 1, ch = wide ? i >> 1 : i, k = cnt + ch, st = k % NS;
-          mbar_wait_bounded(pready + 8 * s, items_s[s] & 1, abort_flag, p.status);
-          ++items_s[s];
-          if (!wide || s == 0) mbar_wait_bounded(vfull + 8 * st, (k / NS) & 1, abort_flag, p.status);
-          fence_after();
-          const uint32_t b = sb + S::kV + st * S::kOperand;
-#pragma unroll
-          for (int kk = 0; kk < kChunk / 16; ++kk)
-            mma_ts(tmem + 256 + s * D, tmem + s * 128 + kk * 8, desc_mnmajor(b + kk * 2048), ID_O,
-                   i >= 2 || kk > 0);
-          if (!wide || s == 1) commit(vempty + 8 * st);
-          if (i + 2 >= items) commit(ofull + 8 * s);
-          if (i + 2 < items) issue_s(i + 2);
+      // Segment entries are read once by each cursor; b's read gives the entry back.
+      auto load = [&](Cursor& c, bool last) {
+        const int slot = c.seg % kRing;
+        mbar_wait_bounded(gfull + 8 * slot, (c.seg / kRing) & 1, abort_flag, p.status);
+        const int4 v = *reinterpret_cast<const int4*>(smem + S::kSegs + 48 * slot);
+        c.n = *abort_flag ? 0 : v.x;
+        c.wide = v.y; c.t0 = v.z; c.hi = v.w;
+        c.j = 0;
+        if (last) mbar_arrive(gempty + 8 * slot);
+        ++c.seg;
+      };
+      auto advance = [&](Cursor& c, bool last) {
+        ++c.item;
+        if (c.wide && c.sub == 0) {
+          c.sub = 1;
+          return;
         }
-        cnt += sg.n;
-        ++nseg;
+        c.sub = 0;
+        ++c.k;
+        if (++c.j == c.n) {
+          c.qc += 1 + c.wide;
+          load(c, last);
+        }
+      };
+      // 32-token blocks of the current chunk that hold tokens
+      auto blocks = [](const Cursor& c) { return (min(kChunk, c.hi - c.t0 - c.j * kChunk) + 31) >> 5; };
+      // V: 16 tokens of a k-step are inside a box, or two boxes of 8 (descriptor units of 16 B)
+      const int vbox = min(p.P, kChunk), vsh = 31 - __clz(vbox), vstep = vbox * 8 * S::kHalves;
+      Cursor a = {}, b = {};     // S (a) runs two items ahead of P V (b)
+      load(a, false);
+      uint32_t ready = 0;        // bit s: parity of stream s's next P
+      auto issue_s = [&]() {
+        const int s = a.item & 1, st = a.k % NS, qi = a.qc + a.sub, qb = qi & 1;
+        if (a.j == 0) mbar_wait_bounded(qfull + 8 * qb, (qi >> 1) & 1, abort_flag, p.status);
+        if (a.sub == 0) mbar_wait_bounded(kfull + 8 * st, (a.k / NS) & 1, abort_flag, p.status);
+        fence_after();
+        const uint64_t qd = desc_kmajor(sb + S::kQ + qb * S::kOperand);
+        const uint64_t kd = desc_kmajor(sb + S::kK + st * S::kOperand);
+        const uint32_t id = ID_S | ((uint32_t)(blocks(a) * 4) << 17);   // N = 32 per block
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = ((kk / 4) * S::kTile + (kk % 4) * 32) >> 4;
+          mma_ss(tmem + s * 128, qd + off, kd + off, id, kk > 0);
+        }
+        commit(sfull + 8 * s);
+        if (!a.wide || a.sub == 1) commit(kempty + 8 * st);
+        if (a.j == a.n - 1) commit(qempty + 8 * qb);
+        advance(a, false);
+      };
+      if (a.n) issue_s();
+      if (a.n) issue_s();
+      load(b, true);
+      while (b.n) {
+        const int s = b.item & 1, st = b.k % NS;
+        mbar_wait_bounded(pready + 8 * s, (ready >> s) & 1, abort_flag, p.status);
+        ready ^= 1u << s;
+        if (b.sub == 0) mbar_wait_bounded(vfull + 8 * st, (b.k / NS) & 1, abort_flag, p.status);
+        fence_after();
+        const uint64_t vd = desc_mnmajor(sb + S::kV + st * S::kOperand, vbox);
+        const bool first = b.wide ? b.j == 0 : b.j < 2;
+        const int nb = blocks(b);
+#pragma unroll
+        for (int kk = 0; kk < kChunk / 16; ++kk)
+          if (kk < 2 * nb)
+            mma_ts(tmem + 256 + s * D, tmem + s * 128 + kk * 8,
+                   vd + (((kk * 16) >> vsh) * vstep + ((kk * 16) & (vbox - 1)) * 8), ID_O,
+                   !first || kk > 0);
+        if (!b.wide || b.sub == 1) commit(vempty + 8 * st);
+        if (b.wide ? b.j == b.n - 1 : b.j >= b.n - 2) commit(ofull + 8 * s);
+        if (a.n) issue_s();
+        advance(b, true);
       }
     }
     __syncwarp();
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---- softmax: thread = query row ----
+    // The first round is a rehearsal on whatever TMEM holds, before any S is issued, while
+    // the tables are built: it brings the code into the instruction caches.  A decode step
+    // streams its weights between two launches, so they are cold (measured: 18 thousand
+    // cycles for the first item without it).
     const int s = warp >> 2, r = tid & 127;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + s * 128, to = tmem + lanes + 256 + s * D;
     const float kNegInf = __int_as_float(0xff800000);
-    const float sc = fabsf(p.scale_log2);
-    const uint32_t flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;   // the sign goes into q
-    int cnt = 0, n_items = 0, n_o = 0;
-    while (next_segment(tp, gr, rt, c, c1, g, sg)) {
-      const int row = (wide ? s * 128 : 0) + r;        // row of the tile
-      const bool warp_on = (wide ? s * 128 : 0) + (warp & 3) * 32 < sg.rows;
-      // Q tile(s) into the swizzled operand layout; stream s loads its tile, or half of
-      // the only one.  A 16-byte vector c of row x sits at x * 128 + ((c ^ x) & 7) * 16.
-      bar_softmax();                                   // the exchange area is free again
-      {
-        constexpr int VPR = D / 8;                     // vectors of a row
-        const uint32_t q0 = sb + S::kQ + (wide ? s * S::kOperand : 0);
-        const int nv = 128 * VPR;
-        const int first = wide ? r : tid, step = wide ? 128 : 256;
-        for (int v = first; v < nv; v += step) {
-          const int x = v / VPR, cv = v - x * VPR;
-          const int qr = (wide ? s * 128 : 0) + x;
-          uint4 val = make_uint4(0u, 0u, 0u, 0u);
-          if (qr < sg.rows) {
-            const int gr_row = sg.tile * rt + qr;
-            const int b = sg.lo + gr_row / p.R, h = sg.hk * p.R + gr_row % p.R;
-            val = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) +
-                                                       ((long long)b * p.Hq + h) * D) + cv);
-            val.x ^= flip; val.y ^= flip; val.z ^= flip; val.w ^= flip;
-          }
-          const uint32_t dst = q0 + (cv >> 3) * S::kTile + x * 128 + (((cv ^ x) & 7) << 4);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(val.x),
-                       "r"(val.y), "r"(val.z), "r"(val.w)
-                       : "memory");
-        }
+    const float sc = p.scale_log2;                     // positive
+    const uint64_t sc2 = pair(sc, sc);
+    const int narrow = tp.nb * p.R;
+    const int box = min(p.P, kChunk), bsh = 31 - __clz(box);
+    int k = 0, it = 0, n_items = 0, n_o = 0;
+    Segment sg;
+    sg.n = 2; sg.wide = 0; sg.t0 = 0; sg.hi = 2 * kChunk - 1; sg.lo = 0; sg.rows = 128; sg.slot = 0;
+    sg.own = 0;
+#pragma unroll 1
+    for (int ns = -1;; ++ns) {
+      const bool real = ns >= 0;
+      if (real) {
+        const int slot = ns % kRing;
+        mbar_wait_bounded(gfull + 8 * slot, (ns / kRing) & 1, abort_flag, p.status);
+        const int4* e = reinterpret_cast<const int4*>(segs + slot);
+        const int4 x = e[0], y = e[1];
+        sg.n = x.x; sg.wide = x.y; sg.t0 = x.z; sg.hi = x.w;
+        sg.lo = y.x; sg.rows = y.y; sg.slot = y.z; sg.own = y.w;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(gempty + 8 * slot);
+        // after a wait that gave up the entry means nothing; a warp leaves as one
+        if (__any_sync(0xffffffffu, sg.n == 0 || *abort_flag != 0)) break;
       }
-      fence_proxy_async_smem();
-      mbar_arrive(qready);
-      const int mine = wide ? sg.n : (sg.n - s + 1) / 2;   // items of this stream
-      float m = kNegInf, l0 = 0.f, l1 = 0.f;
-      for (int i = 0; i < mine; ++i, ++n_items) {
-        const int ch = wide ? i : 2 * i + s;
-        const int t0 = (sg.ch0 + ch) * kChunk;
-        const int valid = min(kChunk, sg.s - t0);
-        mbar_wait_bounded(sfull + 8 * s, n_items & 1, abort_flag, p.status);
+      // q: row tile of this stream (wide), or whether it has the even or the odd chunks.
+      const int q = s ^ (it & 1);
+      const int first = sg.wide ? 0 : q, step = sg.wide ? 1 : 2;
+      const int rows = sg.wide ? min(narrow, sg.rows - q * narrow) : sg.rows;
+      const bool warp_on = (warp & 3) * 32 < rows;
+      float m = kNegInf;
+      uint64_t l2 = pair(0.f, 0.f);
+#pragma unroll 1
+      for (int j = first; j < sg.n; j += step) {
+        const int t0 = sg.t0 + j * kChunk;
+        const int hi = min(kChunk, sg.hi - t0), lo = max(0, sg.lo - t0);
+        const int nb = (hi + 31) >> 5;
+        if (real) mbar_wait_bounded(sfull + 8 * s, n_items & 1, abort_flag, p.status);
         fence_after();
-        if (valid < kChunk && (!wide || s == 0)) {
-          // Rows of V behind the prefix hold anything; a weight 0 would not silence a NaN.
-          // S of this item follows the products of the stream's item before, so the stage's
-          // earlier chunk is done and the wait below cannot take its phase for this one.
-          const int k = cnt + ch, st = k % NS;
-          mbar_wait_bounded(vfull + 8 * st, (k / NS) & 1, abort_flag, p.status);
-          const uint32_t v0 = sb + S::kV + st * S::kOperand;
-          for (int q = r; q < (kChunk - valid) * 8 * S::kHalves; q += 128) {
-            const int h = q / ((kChunk - valid) * 8), w = q - h * (kChunk - valid) * 8;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                             v0 + h * S::kTile + valid * 128 + w * 16),
-                         "r"(0u)
-                         : "memory");
-          }
-          fence_proxy_async_smem();
-        }
         if (warp_on) {
+          // Two passes over S in TMEM, 64 columns at a time: little code, few registers.
           float mx = kNegInf;
 #pragma unroll 1
-          for (int j = 0; j < 4; ++j) {
-            uint32_t v[32];
-            ld32(ts + 32 * j, v);
+          for (int x = 0; x < kChunk; x += 64) {
+            if (x >= 32 * nb) break;
+            uint32_t v[2][32];
+            ld32(ts + x, v[0]);
+            ld32(ts + x + 32, v[1]);     // past nb: old columns, masked
             wait_ld();
-            if (valid == kChunk) {
+            if (x < lo || x + 64 > hi) {   // tokens outside the unit: -inf, also for pass two
 #pragma unroll
-              for (int q = 0; q < 32; ++q) mx = fmaxf(mx, __uint_as_float(v[q]));
-            } else {
-#pragma unroll
-              for (int q = 0; q < 32; ++q)
-                if (32 * j + q < valid) mx = fmaxf(mx, __uint_as_float(v[q]));
+              for (int e = 0; e < 64; ++e)
+                if (x + e < lo || x + e >= hi) v[e / 32][e % 32] = __float_as_uint(kNegInf);
+              st32(ts + x, v[0]);
+              st32(ts + x + 32, v[1]);
+              wait_st();
             }
+            float m0 = kNegInf, m1 = kNegInf;
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              m0 = fmaxf(m0, fmaxf(__uint_as_float(v[0][e]), __uint_as_float(v[0][e + 1])));
+              m1 = fmaxf(m1, fmaxf(__uint_as_float(v[1][e]), __uint_as_float(v[1][e + 1])));
+            }
+            mx = fmaxf(mx, fmaxf(m0, m1));
           }
           // Raise the reference maximum when the weights would pass 2^8.
-          const bool first = i == 0;
-          const bool raise = first || (mx - m) * sc > 8.f;
+          const bool start = j == first;
+          const bool raise = start || (mx - m) * sc > 8.f;
           if (__any_sync(0xffffffffu, raise)) {
             float f = 1.f;
             if (raise) {
-              f = first ? 0.f : ex2((m - mx) * sc);
-              if (m == kNegInf) f = 0.f;
+              f = start || m == kNegInf ? 0.f : ex2((m - mx) * sc);
               m = mx;
-              l0 *= f;
-              l1 *= f;
+              float a, b;
+              unpair(l2, a, b);
+              l2 = pair(a * f, b * f);
             }
-            if (!first) {
+            if (!start) {
 #pragma unroll 1
-              for (int j = 0; j < D / 32; ++j) {
-                uint32_t v[32];
-                ld32(to + 32 * j, v);
+              for (int x = 0; x < D / 16; ++x) {
+                uint32_t o[16];
+                ld16(to + 16 * x, o);
                 wait_ld();
 #pragma unroll
-                for (int q = 0; q < 32; ++q) v[q] = __float_as_uint(__uint_as_float(v[q]) * f);
-                st32(to + 32 * j, v);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                st16(to + 16 * x, o);
               }
             }
           }
           const float ms = m == kNegInf ? 0.f : m * sc;
+          const uint64_t nm2 = pair(-ms, -ms);
 #pragma unroll 1
-          for (int j = 0; j < 4; ++j) {
-            uint32_t v[32], w[16];
-            ld32(ts + 32 * j, v);
+          for (int x = 0; x < kChunk; x += 64) {
+            if (x >= 32 * nb) break;
+            uint32_t v[2][32], w[2][16];
+            ld32(ts + x, v[0]);
+            ld32(ts + x + 32, v[1]);
             wait_ld();
 #pragma unroll
-            for (int q = 0; q < 32; q += 2) {
-              float a = ex2(fmaf(__uint_as_float(v[q]), sc, -ms));
-              float b = ex2(fmaf(__uint_as_float(v[q + 1]), sc, -ms));
-              if (valid < kChunk) {
-                if (32 * j + q >= valid) a = 0.f;
-                if (32 * j + q + 1 >= valid) b = 0.f;
-              }
-              l0 += a;
-              l1 += b;
-              w[q / 2] = Mma<T>::pack(a, b);
+            for (int e = 0; e < 64; e += 2) {
+              float a, b;
+              unpair(fma2(pair(__uint_as_float(v[e / 32][e % 32]),
+                               __uint_as_float(v[e / 32][e % 32 + 1])), sc2, nm2), a, b);
+              a = ex2(a);
+              b = ex2(b);
+              l2 = add2(l2, pair(a, b));
+              w[e / 32][e % 32 / 2] = Mma<T>::pack(a, b);
             }
-            // P's columns 16 j .. 16 j + 15 lie over S's columns of blocks <= j, read above.
-            st16(ts + 16 * j, w);
+            // P's columns x / 2 .. x / 2 + 31 lie over S columns that have been read
+            st16(ts + x / 2, w[0]);
+            st16(ts + x / 2 + 16, w[1]);
           }
           wait_st();
         }
-        fence_before();
-        mbar_arrive(pready + 8 * s);
+        if (real) {
+          if (hi < 32 * nb && (!sg.wide || q == 0)) {
+            // Rows of V behind the last token hold anything; a weight 0 would not silence a
+            // NaN.  S of this item follows the products of the stream's item before, so the
+            // stage's earlier chunk is done: this wait cannot take its phase for the chunk's.
+            const int st = (k + j) % NS;
+            mbar_wait_bounded(vfull + 8 * st, ((k + j) / NS) & 1, abort_flag, p.status);
+            const uint32_t v0 = sb + S::kV + st * S::kOperand;
+            const int per = (32 * nb - hi) * 8;
+#pragma unroll 1
+            for (int i = r; i < per * S::kHalves; i += 128) {
+              const int h = i >= per ? 1 : 0, w = i - h * per, tok = hi + (w >> 3);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                               v0 + (tok >> bsh) * (box * 128 * S::kHalves) + h * (box * 128) +
+                               (tok & (box - 1)) * 128 + (w & 7) * 16),
+                           "r"(0u)
+                           : "memory");
+            }
+            fence_proxy_async_smem();
+          }
+          fence_before();
+          mbar_arrive(pready + 8 * s);
+          ++n_items;
+        }
       }
-      // ---- segment end ----
-      const int slot = sg.unit + (int)blockIdx.x;
-      const int rs = wide ? tp.rs_b : tp.rs_a;
-      float4* po = reinterpret_cast<float4*>(p.part_o) + (long long)slot * rs * (D / 4);
-      float* pl = p.part_lse + (long long)slot * rs;
-      if (mine > 0) {
-        mbar_wait_bounded(ofull + 8 * s, n_o & 1, abort_flag, p.status);
-        ++n_o;
+      // ---- segment end: this stream's partial ----
+      const long long slot = sg.slot + q;
+      const int rs = sg.own ? p.R : tp.rs;
+      float4* po = reinterpret_cast<float4*>(sg.own ? tp.own_o : p.part_o) + slot * rs * (D / 4);
+      float* pl = (sg.own ? tp.own_lse : p.part_lse) + slot * rs;
+      const bool write = real && r < rows;
+      if (first < sg.n) {
+        if (real) {
+          mbar_wait_bounded(ofull + 8 * s, n_o & 1, abort_flag, p.status);
+          ++n_o;
+        }
         fence_after();
-      }
-      float l = l0 + l1;
-      const float ms = m == kNegInf ? 0.f : m * sc;    // log2 units
-      if (wide) {
         if (warp_on) {
+          float a, b;
+          unpair(l2, a, b);
+          const float l = a + b;
           const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll 1
-          for (int j = 0; j < D / 32; ++j) {
-            uint32_t v[32];
-            ld32(to + 32 * j, v);
+          for (int x = 0; x < D / 32; ++x) {
+            uint32_t o[32];
+            ld32(to + 32 * x, o);
             wait_ld();
-            if (row < sg.rows) {
+            if (write) {
 #pragma unroll
-              for (int q = 0; q < 32; q += 4)
-                po[(long long)(8 * j + q / 4) * rs + row] = make_float4(
-                    __uint_as_float(v[q]) * inv, __uint_as_float(v[q + 1]) * inv,
-                    __uint_as_float(v[q + 2]) * inv, __uint_as_float(v[q + 3]) * inv);
+              for (int e = 0; e < 32; e += 4)
+                po[(8 * x + e / 4) * rs + r] = make_float4(
+                    __uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
+                    __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
             }
           }
-          if (row < sg.rows) pl[row] = l == 0.f ? kNegInf : ms + log2f(l);
+          if (write) pl[r] = l == 0.f ? kNegInf : (m == kNegInf ? 0.f : m * sc) + log2f(l);
         }
-      } else {
-        // Each stream finishes half of the columns: it hands the other half of its O over.
-        float* xo = reinterpret_cast<float*>(smem + S::kQ) + s * (D / 2) * 128;
-        ml[s * 128 + r] = make_float2(ms, mine > 0 ? l : 0.f);
-        if (warp_on && mine > 0) {
-#pragma unroll 1
-          for (int j = 0; j < D / 64; ++j) {
-            uint32_t v[32];
-            ld32(to + (1 - s) * (D / 2) + 32 * j, v);
-            wait_ld();
-#pragma unroll
-            for (int q = 0; q < 32; ++q) xo[(32 * j + q) * 128 + r] = __uint_as_float(v[q]);
-          }
-        }
-        bar_softmax();
-        if (warp_on) {
-          const float2 other = ml[(1 - s) * 128 + r];
-          const float lo_ = other.y;
-          const bool have_o = (sg.n - (1 - s) + 1) / 2 > 0;    // the other stream had items
-          const float M = l == 0.f ? other.x : lo_ == 0.f ? ms : fmaxf(ms, other.x);
-          const float wa = l == 0.f ? 0.f : ex2(ms - M), wb = lo_ == 0.f ? 0.f : ex2(other.x - M);
-          const float L = l * wa + lo_ * wb;
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-          const float ia = wa * inv, ib = wb * inv;
-          const float* yo = reinterpret_cast<const float*>(smem + S::kQ) + (1 - s) * (D / 2) * 128;
-#pragma unroll 1
-          for (int j = 0; j < D / 64; ++j) {
-            uint32_t v[32];
-            if (mine > 0) {
-              ld32(to + s * (D / 2) + 32 * j, v);
-              wait_ld();
-            }
-            if (row < sg.rows) {
-#pragma unroll
-              for (int q = 0; q < 32; q += 4) {
-                float o[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  o[e] = mine > 0 ? __uint_as_float(v[q + e]) * ia : 0.f;
-                  if (have_o) o[e] = fmaf(yo[(32 * j + q + e) * 128 + r], ib, o[e]);
-                }
-                po[(long long)(s * (D / 8) + 8 * j + q / 4) * rs + row] =
-                    make_float4(o[0], o[1], o[2], o[3]);
-              }
-            }
-          }
-          if (s == 0 && row < sg.rows) pl[row] = L == 0.f ? kNegInf : M + log2f(L);
-        }
+        fence_before();   // O is read: the next segment's products may overwrite it
+      } else if (write) {
+        pl[r] = kNegInf;  // a single chunk, on the other stream
       }
-      fence_before();   // O is read: the next segment's products may overwrite it
-      cnt += sg.n;
+      if (real) {
+        k += sg.n;
+        it += sg.wide ? 2 * sg.n : sg.n;
+      } else {
+        pdl_wait();       // what follows overwrites partials that the last join may still read
+        fence_before();
+        asm volatile("bar.sync 2, 288;" ::: "memory");
+      }
     }
   }
   fence_before();
@@ -687,284 +1015,73 @@ prefix_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__
 }
 
 // ---------------------------------------------------------------------------------
-// own_kernel: a sequence's own tokens and the join.
-//
-// Block = (token split, KV head and 8 * NH query heads, sequence), four warps, each with
-// 16 tokens at a time and a softmax state of its own.  Nothing is staged in shared memory:
-//   S[heads x tokens] = Q K^T by mma.m16n8k16 with the head-size index permuted, so that a
-//   thread's share of a key row is whole 16-byte vectors (Q is loaded the same way);
-//   O^T[d x heads] += V^T P^T: a thread's vectors of two tokens, interleaved by byte
-//   permutes, are V^T's fragment, again with d permuted (the output index follows), and
-//   P^T's fragment is S's accumulator itself.
-// The splits of a sequence are a cluster; warps, splits and the prefix's partials are
-// joined per output element by the blocks of the cluster together.
-template <int D, int NH>
-struct OwnSmem {
-  static constexpr int kHeads = 8 * NH;
-  static constexpr int kWarps = 4;
-  static constexpr int kO = 0;                                    // [4][heads][D] fp32
-  static constexpr int kMl = kO + kWarps * kHeads * D * 4;        // [4][heads] (max, sum)
-  static constexpr int kInfo = kMl + kWarps * kHeads * 8;         // per head: M, 1 / L
-  static constexpr int kBytes = kInfo + kHeads * 8;
-};
-
-__device__ __forceinline__ uint32_t own_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void own_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
-                   : "memory");
-}
-__device__ __forceinline__ uint32_t own_map(uint32_t a, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ float2 own_ld2(uint32_t a) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 own_ld4(uint32_t a) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(a)
-               : "memory");
-  return v;
-}
-
-template <int D, int NH, typename T>
-__global__ void __launch_bounds__(128) own_kernel(const __grid_constant__ TcParams tp) {
-  using SM = OwnSmem<D, NH>;
-  constexpr int HEADS = SM::kHeads;
-  constexpr int NK = D / 32;     // 16-byte vectors of a key row per thread
-  constexpr int NV = D / 64;     // of a value row per thread
+// join_kernel: D / 4 lanes per output row, each with 4 of its elements.  The lanes first
+// share the parts' log2-sum-exps (a part each), then all run over the parts.
+template <int D, typename T>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TcParams tp) {
+  constexpr int LPR = D / 4;
   const Params& p = tp.p;
-  __shared__ __align__(16) uint8_t sm[SM::kBytes];
-  __shared__ int scratch[2];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gq = lane >> 2, t4 = lane & 3;
-  const int ns = gridDim.x, split = blockIdx.x;
-  const int hgs = (p.R + HEADS - 1) / HEADS;
-  const int hk = blockIdx.y / hgs, hg = blockIdx.y - hk * hgs;
-  const int b = blockIdx.z;
-  const int h0 = hk * p.R + hg * HEADS;                  // first query head
-  const int nh = min(HEADS, p.R - hg * HEADS);
-  const float kNegInf = __int_as_float(0xff800000);
   pdl_launch_dependents();
-  // Everything up to the join reads only what was final before prefix_kernel let this
-  // kernel start (it does so behind its own wait for its predecessors).
-
-  const int g = group_of(p, b, scratch);
-  int s = 0, lo = 0;
-  if (g >= 0) {
-    int hi, leader;
-    group_range(p, g, lo, hi);
-    group_prefix(p, g, lo, hi, scratch, s, leader);
-  }
-  const int len = seq_len(p, b, split == 0 && tid == 0);
-  bool shared = s > 0 && len > 0;
-  const int t_begin = min(s, len);
-
-  // Q: rows gq and gq + 8 of the m16 tile are heads of this block.
-  uint32_t qa[2 * NK][4];
-  {
-    const T* q = reinterpret_cast<const T*>(p.q) + ((long long)b * p.Hq + h0) * D;
+  pdl_wait();
+  const int lane = threadIdx.x & (LPR - 1);
+  const long long row = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const unsigned mask = LPR == 32 ? 0xffffffffu
+                                  : 0xffffu << (threadIdx.x & 16);
+  if (row >= (long long)p.B * p.Hq) return;
+  const int hkr = quot((int)row, p.R), rh = (int)row - hkr * p.R;   // (b, KV head), head
+  const int4 v = tp.plan[hkr];
+  const float kNegInf = __int_as_float(0xff800000);
+  float M = kNegInf, L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  // The parts of a unit: slots first, first + 1, ... or every second of them.
+  auto add = [&](const float* lse, const float4* o, int rs, int parts, int step) {
+    for (int e0 = 0; e0 < parts; e0 += LPR) {
+      const int n = min(LPR, parts - e0);
+      const float mine = lane < n ? lse[(long long)(e0 + lane) * step * rs] : kNegInf;
+      float top = mine;
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
-      uint4 x = make_uint4(0u, 0u, 0u, 0u), y = x;
-      if (gq < nh) x = __ldg(reinterpret_cast<const uint4*>(q + gq * D) + i * 4 + t4);
-      if (NH == 2 && gq + 8 < nh)
-        y = __ldg(reinterpret_cast<const uint4*>(q + (gq + 8) * D) + i * 4 + t4);
-      qa[2 * i][0] = x.x; qa[2 * i][2] = x.y; qa[2 * i + 1][0] = x.z; qa[2 * i + 1][2] = x.w;
-      qa[2 * i][1] = y.x; qa[2 * i][3] = y.y; qa[2 * i + 1][1] = y.z; qa[2 * i + 1][3] = y.w;
-    }
-  }
-  float m[NH], l[NH], o[NH][D / 16][4];
+      for (int x = LPR / 2; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, x, LPR));
+      const float nm = fmaxf(M, top);
+      const float mu = nm == kNegInf ? 0.f : nm;
+      const float f = ex2(M - mu);
+      M = nm;
+      L *= f;
+      acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+      const float wm = ex2(mine - mu);
+      const float4* src = o + (long long)e0 * step * rs * (D / 4);
+      for (int e1 = 0; e1 < n; e1 += 8) {   // eight parts' loads in flight
+        float4 x[8];
 #pragma unroll
-  for (int a = 0; a < NH; ++a) {
-    m[a] = kNegInf;
-    l[a] = 0.f;
+        for (int e = 0; e < 8; ++e)
+          if (e1 + e < n) x[e] = src[(long long)(e1 + e) * step * rs * (D / 4)];
 #pragma unroll
-    for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[a][j][e] = 0.f;
-  }
-  const T* kp = reinterpret_cast<const T*>(p.k_pages);
-  const T* vp = reinterpret_cast<const T*>(p.v_pages);
-  const int32_t* row = p.block_table + (long long)b * p.max_pages;
-  const int stride = 16 * 4 * ns;
-  for (int t0 = t_begin + 16 * (split * 4 + warp); t0 < len; t0 += stride) {
-    // Rows of this thread: keys t0 + gq, t0 + gq + 8; values t0 + {2 t4, 2 t4 + 1, + 8, + 9}.
-    auto base_of = [&](int tok) -> long long {
-      int page = row[tok / p.P];
-      if (page < 0 || page >= p.num_pages) {
-        atomicOr(p.status, kStatusBadPage);
-        page = 0;
-      }
-      return (((long long)page * p.Hkv + hk) * p.P + tok % p.P) * D;
-    };
-    uint4 kx[2][NK], vx[4][NV];
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      const int tok = t0 + gq + 8 * a;
-#pragma unroll
-      for (int i = 0; i < NK; ++i) kx[a][i] = make_uint4(0u, 0u, 0u, 0u);
-      if (tok < len) {
-        const uint4* src = reinterpret_cast<const uint4*>(kp + base_of(tok)) + t4;
-#pragma unroll
-        for (int i = 0; i < NK; ++i) kx[a][i] = __ldg(src + i * 4);
-      }
-    }
-#pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      const int tok = t0 + 2 * t4 + (a & 1) + 8 * (a >> 1);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) vx[a][i] = make_uint4(0u, 0u, 0u, 0u);
-      if (tok < len) {
-        const uint4* src = reinterpret_cast<const uint4*>(vp + base_of(tok)) + gq;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) vx[a][i] = __ldg(src + i * 8);
-      }
-    }
-    float sc[2][4];
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sc[a][e] = 0.f;
-#pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        Mma<T>::run(sc[a], qa[2 * i], kx[a][i].x, kx[a][i].y);
-        Mma<T>::run(sc[a], qa[2 * i + 1], kx[a][i].z, kx[a][i].w);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)   // tokens t0 + 8 a + 2 t4 + (e & 1)
-        sc[a][e] = t0 + 8 * a + 2 * t4 + (e & 1) < len ? sc[a][e] * p.scale_log2 : kNegInf;
-    }
-#pragma unroll
-    for (int a = 0; a < NH; ++a) {
-      // heads gq + 8 a
-      float tm = fmaxf(fmaxf(sc[0][2 * a], sc[0][2 * a + 1]), fmaxf(sc[1][2 * a], sc[1][2 * a + 1]));
-      tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 1));
-      tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
-      const float mn = fmaxf(m[a], tm);
-      const float mu = mn == kNegInf ? 0.f : mn;
-      const float f = ex2(m[a] - mu);
-      m[a] = mn;
-      const float p0 = ex2(sc[0][2 * a] - mu), p1 = ex2(sc[0][2 * a + 1] - mu);
-      const float p2 = ex2(sc[1][2 * a] - mu), p3 = ex2(sc[1][2 * a + 1] - mu);
-      l[a] = l[a] * f + ((p0 + p1) + (p2 + p3));
-      const uint32_t b0 = Mma<T>::pack(p0, p1), b1 = Mma<T>::pack(p2, p3);
-      if (__any_sync(0xffffffffu, f != 1.f)) {
-        const float f0 = __shfl_sync(0xffffffffu, f, 8 * t4), f1 = __shfl_sync(0xffffffffu, f, 8 * t4 + 4);
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j) {
-          o[a][j][0] *= f0; o[a][j][1] *= f1; o[a][j][2] *= f0; o[a][j][3] *= f1;
+        for (int e = 0; e < 8; ++e) {
+          const float w = __shfl_sync(mask, wm, (e1 + e) & (LPR - 1), LPR);
+          if (e1 + e >= n || w == 0.f) continue;   // an empty part's O is not written
+          L += w;
+          acc.x = fmaf(x[e].x, w, acc.x); acc.y = fmaf(x[e].y, w, acc.y);
+          acc.z = fmaf(x[e].z, w, acc.z); acc.w = fmaf(x[e].w, w, acc.w);
         }
       }
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        const int i = j / 4, w = j % 4;
-        auto word = [&](const uint4& v) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; };
-        uint32_t af[4];
-        af[0] = __byte_perm(word(vx[0][i]), word(vx[1][i]), 0x5410);
-        af[1] = __byte_perm(word(vx[0][i]), word(vx[1][i]), 0x7632);
-        af[2] = __byte_perm(word(vx[2][i]), word(vx[3][i]), 0x5410);
-        af[3] = __byte_perm(word(vx[2][i]), word(vx[3][i]), 0x7632);
-        Mma<T>::run(o[a][j], af, b0, b1);
-      }
     }
+  };
+  if (v.z) {
+    const long long slot = v.x;
+    const int tr = ((v.z >> 16) & 0x7fff) + rh;
+    add(p.part_lse + slot * tp.rs + tr,
+        reinterpret_cast<const float4*>(p.part_o) + (slot * (D / 4) + lane) * tp.rs + tr, tp.rs,
+        v.z & 0xffff, v.z < 0 ? 2 : 1);
   }
-  // ---- this warp's state into shared memory ----
-  float* so = reinterpret_cast<float*>(sm + SM::kO) + warp * HEADS * D;
-  float2* sml = reinterpret_cast<float2*>(sm + SM::kMl) + warp * HEADS;
-#pragma unroll
-  for (int a = 0; a < NH; ++a) {
-    float ls = l[a];
-    ls += __shfl_xor_sync(0xffffffffu, ls, 1);
-    ls += __shfl_xor_sync(0xffffffffu, ls, 2);
-    if (t4 == 0) sml[8 * a + gq] = make_float2(m[a], ls);
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) {
-      // rows gq, gq + 8 of the m-tile are d, d + 1; columns are heads 2 t4, 2 t4 + 1
-      const int d = (j / 4) * 64 + gq * 8 + 2 * (j % 4);
-      *reinterpret_cast<float2*>(so + (8 * a + 2 * t4) * D + d) = make_float2(o[a][j][0], o[a][j][2]);
-      *reinterpret_cast<float2*>(so + (8 * a + 2 * t4 + 1) * D + d) = make_float2(o[a][j][1], o[a][j][3]);
-    }
+  if (v.w) {
+    const long long slot = v.y;
+    add(tp.own_lse + slot * p.R + rh,
+        reinterpret_cast<const float4*>(tp.own_o) + (slot * (D / 4) + lane) * p.R + rh, p.R, v.w, 1);
   }
-  // ---- join: warps and splits of the cluster, then the prefix's partials ----
-  if (ns > 1) own_cluster_sync(); else __syncthreads();
-  pdl_wait();   // prefix_kernel's partials and plan
-  const uint32_t a_o = smem_u32(sm + SM::kO), a_ml = smem_u32(sm + SM::kMl);
-  int first = 0, nseg = 0, W = 0, rt = 128, rs = 1, unit0 = 0, start = 0, nch = 0, tiles = 1;
-  if (shared) {
-    W = tp.plan[0];
-    rt = tp.plan[1];
-    const int4 v = reinterpret_cast<const int4*>(tp.plan + 8)[g];
-    start = v.x; unit0 = v.y; nch = v.z;
-    shared = nch > 0;   // bad groups (reported): prefix_kernel has left nothing
-    tiles = (v.w + rt - 1) / rt;
-    rs = rt == 256 ? tp.rs_b : tp.rs_a;
-  }
-  // A thread makes 4 elements of a head at a time, the blocks of a cluster share the heads.
-  const int items = nh * (D / 4);
-  for (int it = split * 128 + tid; it < items; it += ns * 128) {
-    const int h = it / (D / 4), d4 = it - h * (D / 4);
-    float M = kNegInf;
-    for (int e = 0; e < 4 * ns; ++e) {
-      const float2 v = own_ld2(own_map(a_ml + ((e & 3) * HEADS + h) * 8, e >> 2));
-      if (v.y != 0.f) M = fmaxf(M, v.x);
-    }
-    long long slot0 = 0;
-    if (shared) {
-      const int rr = (b - lo) * p.R + hg * HEADS + h;      // row of the group
-      const int tile = rr / rt, u = hk * tiles + tile;
-      const int ustart = start + u * nch;
-      const int C = min(tp.ctas, W);
-      first = cta_owner(ustart, W, C);
-      nseg = cta_owner(ustart + nch - 1, W, C) - first + 1;
-      slot0 = (long long)(unit0 + u + first);
-      const float* pl = p.part_lse + slot0 * rs + (rr - tile * rt);
-#pragma unroll 4
-      for (int e = 0; e < nseg; ++e) M = fmaxf(M, pl[(long long)e * rs]);
-    }
-    float L = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float mu = M == kNegInf ? 0.f : M;
-    for (int e = 0; e < 4 * ns; ++e) {
-      const float2 v = own_ld2(own_map(a_ml + ((e & 3) * HEADS + h) * 8, e >> 2));
-      if (v.y == 0.f) continue;
-      const float w = ex2(v.x - mu);
-      const float4 x = own_ld4(own_map(a_o + (((e & 3) * HEADS + h) * D + d4 * 4) * 4, e >> 2));
-      L = fmaf(v.y, w, L);
-      acc.x = fmaf(x.x, w, acc.x); acc.y = fmaf(x.y, w, acc.y);
-      acc.z = fmaf(x.z, w, acc.z); acc.w = fmaf(x.w, w, acc.w);
-    }
-    if (shared) {
-      const int rr = (b - lo) * p.R + hg * HEADS + h;
-      const int tr = rr - rr / rt * rt;
-      const float* pl = p.part_lse + slot0 * rs + tr;
-      const float4* po = reinterpret_cast<const float4*>(p.part_o) +
-                         (slot0 * (D / 4) + d4) * rs + tr;
-#pragma unroll 4
-      for (int e = 0; e < nseg; ++e) {
-        const float w = ex2(pl[(long long)e * rs] - mu);   // an empty part: 2^-inf = 0
-        const float4 x = po[(long long)e * rs * (D / 4)];
-        L += w;
-        acc.x = fmaf(x.x, w, acc.x); acc.y = fmaf(x.y, w, acc.y);
-        acc.z = fmaf(x.z, w, acc.z); acc.w = fmaf(x.w, w, acc.w);
-      }
-    }
-    const float inv = L == 0.f ? 0.f : 1.f / L;     // an empty sequence gives zeros
-    uint2 r;
-    r.x = Mma<T>::pack(acc.x * inv, acc.y * inv);
-    r.y = Mma<T>::pack(acc.z * inv, acc.w * inv);
-    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + ((long long)b * p.Hq + h0 + h) * D +
-                              d4 * 4) = r;
-  }
-  if (ns > 1) own_cluster_sync();   // the peers have read this block's shared memory
+  const float inv = L == 0.f ? 0.f : 1.f / L;     // an empty sequence gives zeros
+  uint2 r;
+  r.x = Mma<T>::pack(acc.x * inv, acc.y * inv);
+  r.y = Mma<T>::pack(acc.z * inv, acc.w * inv);
+  reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + row * D)[lane] = r;
 }
 
 }  // namespace tc

@@ -346,3 +346,11 @@ def test_many_units_per_block_narrow_heads():
                                 for j in range(3)], 16, 4, 64, 32, HF, seed=14)
     for _ in range(3):
         b.check(b.run(max_group=3))
+
+
+def test_batch_whose_tables_do_not_fit_shared_memory():
+    sizes = [1 + i % 5 for i in range(1200)]
+    shared = [(7 * i) % 40 for i in range(1200)]
+    lens = [shared[g] + (3 * g + j) % 9 for g, n in enumerate(sizes) for j in range(n)]
+    b = Batch(sizes, shared, lens, 2, 1, 128, 16, BF, seed=15)
+    b.check(b.run(max_group=5))
