@@ -5,16 +5,21 @@
 // over its K beams and the vocabulary, in descending order, ties to the lowest k * V + v.
 // One launch and no global workspace: a thread-block cluster owns a prompt and cuts its
 // K rows into tasks (row, split).  A task is one pass over its logits: every thread keeps
-// a running maximum and sum of exponentials, every warp the n best logits it has seen (a
-// threshold and a short list in shared memory, so an element usually costs one compare).
-// The order inside a row is that of its logits, which needs no log-sum-exp, so one pass is
-// enough.  The CTA merges its warps' lists by rank, the cluster's first CTA collects all
-// lists and sums through distributed shared memory and ranks the candidates by their
-// scores.  Bound: the logits are read once from HBM.
+// a running maximum and sum of exponentials, and the maximum of each of its cells (32
+// elements, more in long rows) in shared memory.  The order inside a row is that of its
+// logits, which needs no log-sum-exp, so the n best can be found before it is known: at
+// least n elements reach the n-th largest of the (pairs of) threads' maxima, and only the
+// few cells that reach it are read again.  Ranks come from comparing all pairs of the few survivors
+// (rows of very many equal logits go through sorted lists instead).  The cluster's first
+// CTA fetches the tasks' lists and sums through distributed shared memory and ranks the
+// candidates by their scores in the same way.
+// Bound: the logits are read once from HBM; then the exponentials (16 a cycle and SM).
+// Measured before the cells, with lists kept up to date while streaming: 104 us for 131 MB
+// of logits, of which the exponentials were a fifth.
 //
-// Sums of exponentials are held in fp32 per thread and joined in fp64; scores are ranked
-// in fp64 (candidates of different beams are often closer than fp32 tells apart) and
-// rounded once to fp32.
+// Sums of exponentials are held in fp32 per thread, joined in fp32 inside a split and in
+// fp64 across splits; scores are ranked in fp64 (candidates of different beams are often
+// closer than fp32 tells apart) and rounded once to fp32.
 //
 // beam_reorder: beam i of a prompt continues from beam parent[i].  See below.
 #include <climits>
@@ -28,7 +33,8 @@ namespace beam {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxBeams = 32;
-constexpr int kU = 4;           // 16-byte vectors a lane has in flight
+constexpr int kU = 4;           // 16-byte vectors of a tile per lane; two more tiles in flight
+constexpr int kCells = 32;      // cells of a thread
 
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;
@@ -144,26 +150,168 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two fp32 operations at once.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// The words of a vector: elements per word, their values, the larger of two words by element.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) beam_select_kernel(const SelectParams p) {
-  constexpr int VEC = 16 / sizeof(T);
+struct Word;
+template <>
+struct Word<float> {
+  static constexpr int kN = 1;
+  static constexpr uint32_t kNegInf = 0xff800000u;
+  static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+  static __device__ __forceinline__ float top(uint32_t a) { return __uint_as_float(a); }
+  static __device__ __forceinline__ float get(uint32_t a, int) { return __uint_as_float(a); }
+};
+template <>
+struct Word<__half> {
+  static constexpr int kN = 2;
+  static constexpr uint32_t kNegInf = 0xfc00fc00u;
+  static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+    const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ float get(uint32_t a, int e) {
+    return __half2float(__ushort_as_half((unsigned short)(e ? a >> 16 : a & 0xffffu)));
+  }
+  static __device__ __forceinline__ float top(uint32_t a) { return fmaxf(get(a, 0), get(a, 1)); }
+};
+template <>
+struct Word<__nv_bfloat16> {
+  static constexpr int kN = 2;
+  static constexpr uint32_t kNegInf = 0xff80ff80u;
+  static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a),
+                                     *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ float get(uint32_t a, int e) {
+    return __uint_as_float(e ? a & 0xffff0000u : a << 16);
+  }
+  static __device__ __forceinline__ float top(uint32_t a) { return fmaxf(get(a, 0), get(a, 1)); }
+};
+
+// How many of the n descending entries of a are better than `key`.
+__device__ __forceinline__ int count_better(const unsigned long long* a, int n,
+                                            unsigned long long key) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (a[mid] > key) lo = mid + 1; else hi = mid;
+  }
+  return lo;
+}
+
+// Merges the warps' sorted lists (buf[w * kCap], len[w] entries) into the n best, in out;
+// the rest of out is 0.  tmp: 6 * n keys, tlen: 6 lengths.  All threads of the block.
+// In pairs: an element's rank is its place plus a binary search in the other list.
+__device__ __noinline__ void merge_warps(const unsigned long long* buf, const int* len, int n,
+                                         unsigned long long* tmp, int* tlen,
+                                         unsigned long long* out) {
+  const int tid = threadIdx.x;
+  for (int i = tid; i < n; i += kThreads) out[i] = 0ull;
+  __syncthreads();
+  for (int level = 0; level < 3; ++level) {
+    const int pairs = 4 >> level;
+    // level 0: the warps' lists -> tmp[0..3], level 1: -> tmp[4..5], level 2: -> out
+    const unsigned long long* src = level == 0 ? buf : level == 1 ? tmp : tmp + 4 * n;
+    const int stride = level == 0 ? kCap : n;
+    const int* sl = level == 0 ? len : level == 1 ? tlen : tlen + 4;
+    unsigned long long* dst = level == 2 ? out : level == 0 ? tmp : tmp + 4 * n;
+    for (int i = tid; i < pairs * 2 * n; i += kThreads) {
+      const int w = i / n, j = i - w * n;       // list, place
+      if (j >= sl[w]) continue;
+      const unsigned long long key = src[w * stride + j];
+      const int r = j + count_better(src + (w ^ 1) * stride, sl[w ^ 1], key);
+      if (r < n) dst[(w >> 1) * n + r] = key;
+    }
+    if (level < 2 && tid < pairs)
+      tlen[4 * level + tid] = min(n, sl[2 * tid] + sl[2 * tid + 1]);
+    __syncthreads();
+  }
+}
+
+// A candidate: its fp64 score as bits that order like it, and beam << 32 | token, of which
+// the lower is better.
+struct __align__(16) Cand {
+  unsigned long long score, tie;
+};
+__device__ __forceinline__ unsigned long long score_bits(double x) {
+  const unsigned long long u = (unsigned long long)__double_as_longlong(x + 0.0);   // no -0
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double bits_score(unsigned long long u) {
+  return __longlong_as_double((long long)(u >> 63 ? u & ~(1ull << 63) : ~u));
+}
+__device__ __forceinline__ bool better(const Cand& a, const Cand& b) {
+  return a.score > b.score || (a.score == b.score && a.tie < b.tie);
+}
+
+// Candidates of the merge space: half the lists, or what all pairs are compared of.
+__host__ __device__ inline int spare_cands(int n, int tasks) {
+  const int halved = (tasks + 1) / 2 * n, most = tasks * n < kThreads ? tasks * n : kThreads;
+  return halved > most ? halved : most;
+}
+// Bytes of dynamic shared memory (see the kernel).
+__host__ __device__ inline size_t select_smem(int K, int n, int tasks, int per_cta) {
+  const size_t keys = (size_t)kWarps * kCap + 6 * (size_t)n + (size_t)per_cta * (n + 1) +
+                      (size_t)tasks * (n + 1) + (size_t)kCells * kThreads / 2;
+  const size_t cands = (size_t)tasks * n + spare_cands(n, tasks);
+  return (keys + (keys & 1)) * 8 + cands * sizeof(Cand) + (size_t)K * 24;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectParams p) {
+  constexpr int VEC = 16 / sizeof(T), WN = Word<T>::kN;
   extern __shared__ __align__(16) uint8_t sm_raw[];
   const int n = p.n, K = p.K, V = p.V, S = p.splits;
   const uint32_t rank = cluster_ctarank(), C = cluster_nctarank();
   const int g = blockIdx.x / C;
   const int tasks = K * S;
   const int per_cta = (tasks + (int)C - 1) / (int)C;
-  // shared: warp buffers [kWarps][kCap], this CTA's lists [per_cta][n], sums [per_cta],
-  // then (first CTA) all lists [tasks][n], row constants.
+  // shared: warp buffers [kWarps][kCap], merge space [6][n], this CTA's lists [per_cta][n]
+  // and sums [per_cta], cells [kCells][kThreads]; then (first CTA) all lists [tasks][n] and
+  // sums, the candidates and their merge space, row constants.
   unsigned long long* wbuf = reinterpret_cast<unsigned long long*>(sm_raw);
-  unsigned long long* lists = wbuf + kWarps * kCap;
+  unsigned long long* tmp = wbuf + kWarps * kCap;
+  unsigned long long* lists = tmp + 6 * n;
   unsigned long long* sums = lists + (size_t)per_cta * n;       // (max, sum) as two floats
-  unsigned long long* all = sums + per_cta;
-  double* row_lse = reinterpret_cast<double*>(all + (size_t)tasks * n);
+  float* cells = reinterpret_cast<float*>(sums + per_cta);
+  unsigned long long* all = sums + per_cta + kCells * kThreads / 2;
+  unsigned long long* all_sums = all + (size_t)tasks * n;
+  const size_t keys = (size_t)kWarps * kCap + 6 * n + (size_t)per_cta * (n + 1) +
+                      (size_t)tasks * (n + 1) + kCells * kThreads / 2;
+  Cand* cand = reinterpret_cast<Cand*>(wbuf + keys + (keys & 1));
+  Cand* half = cand + (size_t)tasks * n;
+  double* row_lse = reinterpret_cast<double*>(half + spare_cands(n, tasks));
   double* row_b = row_lse + K;
   int* row_kind = reinterpret_cast<int*>(row_b + K);            // 0 live, 1 dead, 2 finished
-  __shared__ float red_m[kWarps], red_s[kWarps];
-  __shared__ int wcount[kWarps];
+  __shared__ float red_m[kWarps], red_s[kWarps], red_b[kWarps];
+  __shared__ __align__(16) float maxima[kThreads / 2];
+  __shared__ int hits[kThreads];
+  __shared__ int wcount[kWarps], tlen[6], n_hits, survivors;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
@@ -171,6 +319,7 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const SelectParam
 
   constexpr float kLog2e = 1.4426950408889634f;
   const float kNegInf = __int_as_float(0xff800000);
+  const uint64_t l2e = pair(kLog2e, kLog2e);
 
   for (int t = (int)rank, slot = 0; t < tasks; t += (int)C, ++slot) {
     const int row = t / S, split = t - row * S;
@@ -189,103 +338,110 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const SelectParam
     // A warp's vectors are contiguous, so its later elements have larger indices.
     const int w0 = v0 + (int)((long long)(v1 - v0) * warp / kWarps);
     const int w1 = v0 + (int)((long long)(v1 - v0) * (warp + 1) / kWarps);
-    WarpTop top;
-    top.buf = wbuf + warp * kCap;
-    top.n = n;
-    top.count = 0;
-    top.tau = kNegInf;
-    top.full = false;
-    float m = kNegInf, s = 0.f;
-    bool nan = false;
-    for (int base = w0; base < w1; base += 32 * kU) {
-      uint4 raw[kU];
+    // Tiles of whole vectors of this warp's part: [whole0, whole1).
+    const uint4* vec = reinterpret_cast<const uint4*>(x - h) + lane;
+    const int whole0 = h ? 1 : 0, whole1 = min(w1, (V + h) / VEC);
+    auto load = [&](int base, uint4 (&raw)[kU]) {
+      if (base >= whole0 && base + 32 * kU <= whole1) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) raw[u] = __ldg(vec + base + u * 32);
+        return;
+      }
+      // the ends of a row, or past this warp's part: -inf outside
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
         const int v = base + u * 32 + lane;
         const long long e0 = (long long)v * VEC - h;
-        T* r = reinterpret_cast<T*>(&raw[u]);
-        if (v < w1 && e0 >= 0 && e0 + VEC <= V) {
-          raw[u] = __ldg(reinterpret_cast<const uint4*>(x + e0));
-        } else {   // the ends of a row, or past this warp's part: -inf outside
+        constexpr uint32_t F = Word<T>::kNegInf;
+        raw[u] = make_uint4(F, F, F, F);
+        if (v >= w1) continue;
+        if (v >= whole0 && v < whole1) {
+          raw[u] = __ldg(vec + base + u * 32);
+        } else {
+          T* r = reinterpret_cast<T*>(&raw[u]);
 #pragma unroll
           for (int e = 0; e < VEC; ++e)
-            r[e] = (v < w1 && e0 + e >= 0 && e0 + e < V) ? x[e0 + e] : from_f32<T>(kNegInf);
+            if (e0 + e >= 0 && e0 + e < V) r[e] = x[e0 + e];
         }
       }
-      float tile_m = kNegInf;
+    };
+    // One pass: maximum, sum, cells.
+    float m = kNegInf, ml = 0.f;     // ml = m log2(e), rounded; 0 while m = -inf
+    uint64_t s2 = pair(0.f, 0.f);
+    // tiles of a cell, the same for all warps
+    const int tiles = ((v1 - v0 + kWarps - 1) / kWarps + 32 * kU - 1) / (32 * kU);
+    const int per_cell = (tiles + kCells - 1) / kCells;
+    float cell_m = kNegInf;
+    int in_cell = 0, cell = 0;
+    uint4 cur[kU], ahead[kU];
+    load(w0, cur);
+    load(w0 + 32 * kU, ahead);
+    for (int base = w0; base < w1; base += 32 * kU) {
+      uint4 next[kU];
+      load(base + 64 * kU, next);
+      const uint32_t* wd = reinterpret_cast<const uint32_t*>(cur);
+      uint32_t mw = wd[0];
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const T* r = reinterpret_cast<const T*>(&raw[u]);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) tile_m = fmaxf(tile_m, to_f32(r[e]));
+      for (int i = 1; i < kU * 4; ++i) mw = Word<T>::max(mw, wd[i]);
+      const float tile_m = Word<T>::top(mw);
+      cell_m = fmaxf(cell_m, tile_m);
+      if (++in_cell == per_cell || base + 32 * kU >= w1) {
+        cells[cell * kThreads + threadIdx.x] = cell_m;
+        cell_m = kNegInf;
+        in_cell = 0;
+        ++cell;
       }
-      // running maximum and sum of this thread
+      // The exponent x log2(e) - ml is one fused operation; ml's rounding is common to all
+      // terms and taken out at the end.
       if (tile_m > m) {
-        s *= ex2((m - tile_m) * kLog2e);   // m = -inf: s is 0
+        const float nl = tile_m * kLog2e, f = ex2(ml - nl);
+        const float2 o = unpair(s2);
+        s2 = m == kNegInf ? s2 : pair(o.x * f, o.y * f);
         m = tile_m;
+        ml = nl;
       }
-      const float mm = m == kNegInf ? 0.f : m;
+      const uint64_t nml = pair(-ml, -ml);
+#pragma unroll
+      for (int i = 0; i < kU * 4; i += 3 - WN) {
+        const float a = Word<T>::get(wd[i], 0);
+        const float b = WN == 2 ? Word<T>::get(wd[i], 1) : Word<T>::get(wd[i + 1], 0);
+        const float2 e = unpair(fma2(pair(a, b), l2e, nml));
+        s2 = add2(s2, pair(ex2(e.x), ex2(e.y)));
+      }
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
-        const T* r = reinterpret_cast<const T*>(&raw[u]);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) s += ex2((to_f32(r[e]) - mm) * kLog2e);
+        cur[u] = ahead[u];
+        ahead[u] = next[u];
       }
-      nan |= s != s;
-      // The n best: nothing to do unless some lane's largest value passes.
-      if (top.full && !__any_sync(0xffffffffu, tile_m > top.tau)) continue;
-      // Before the list is full, the n-th largest lane maximum bounds the tile's n-th best.
-      const float lo = top.full ? top.tau : (n <= 32 ? nth_lane_max(tile_m, n, lane) : kNegInf);
-      uint32_t mask = 0;
-#pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const int v = base + u * 32 + lane;
-        const T* r = reinterpret_cast<const T*>(&raw[u]);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const long long i = (long long)v * VEC - h + e;
-          const float f = to_f32(r[e]);
-          const bool pass = (top.full ? f > lo : f >= lo) && v < w1 && i >= 0 && i < V;
-          mask |= pass ? 1u << (u * VEC + e) : 0u;
-        }
-      }
-      while (true) {
-        bool pass = mask != 0;
-        unsigned vote = __ballot_sync(0xffffffffu, pass);
-        if (!vote) break;
-        const int bit = pass ? __ffs(mask) - 1 : 0;
-        mask &= mask - 1;
-        float f = 0.f;
-#pragma unroll
-        for (int q = 0; q < kU * VEC; ++q)
-          if (q == bit) f = to_f32(reinterpret_cast<const T*>(&raw[q / VEC])[q % VEC]);
-        if (top.count + __popc(vote) > kCap) {
-          // Elements of this tile are in no order: equal values still compete by index.
-          top_compact(top, lane);
-          pass = pass && (!top.full || f >= top.tau);
-          vote = __ballot_sync(0xffffffffu, pass);
-        }
-        const int v = base + (bit / VEC) * 32 + lane;
-        if (pass)
-          top.buf[top.count + __popc(vote & ((1u << lane) - 1u))] =
-              make_key(f, (uint32_t)((long long)v * VEC - h + bit % VEC));
-        top.count += __popc(vote);
-      }
-      if (!top.full && top.count >= n) top_compact(top, lane);
     }
-    top_compact(top, lane);
-    // join the warps: maximum and sum, then the lists
-    if (nan) s = __int_as_float(0x7fc00000);   // a NaN, or an infinity, among the logits
+    // Join the maxima and sums, and the bound on the n-th best.
+    const float2 sp = unpair(s2);
+    float s = sp.x + sp.y;               // NaN: a NaN, or an infinity, among the logits
     float wm = m;
     for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-    float ws = m == kNegInf ? s : s * ex2((m - wm) * kLog2e);
+    // 2^((m - wm) log2(e)), and ml's rounding taken out
+    float ws = m == kNegInf ? s : s * ex2((m - wm) * kLog2e - fmaf(m, kLog2e, -ml));
     for (int o = 16; o; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
+    const float m2 = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));   // of two threads
+    if (!(lane & 1)) maxima[threadIdx.x >> 1] = m2;
     if (lane == 0) {
       red_m[warp] = wm;
       red_s[warp] = ws;
-      wcount[warp] = top.count;
     }
+    if (threadIdx.x == 0) n_hits = survivors = 0;
     __syncthreads();
+    // The n-th largest of the maxima of two threads: the least of those that fewer than n
+    // exceed.  Each of the two counts in one half.
+    int above = 0;
+#pragma unroll 4
+    for (int i = (lane & 1) * (kThreads / 4), e = i + kThreads / 4; i < e; i += 4) {
+      const float4 o = *reinterpret_cast<const float4*>(maxima + i);
+      above += (o.x > m2) + (o.y > m2) + (o.z > m2) + (o.w > m2);
+    }
+    above += __shfl_xor_sync(0xffffffffu, above, 1);
+    float wb = above < n ? m2 : __int_as_float(0x7f800000);
+    for (int o = 16; o; o >>= 1) wb = fminf(wb, __shfl_xor_sync(0xffffffffu, wb, o));
+    if (lane == 0) red_b[warp] = wb;
     if (threadIdx.x == 0) {
       float M = kNegInf;
       for (int w = 0; w < kWarps; ++w) M = fmaxf(M, red_m[w]);
@@ -294,123 +450,221 @@ __global__ void __launch_bounds__(kThreads) beam_select_kernel(const SelectParam
         sum += red_m[w] == kNegInf ? red_s[w] : red_s[w] * ex2((red_m[w] - M) * kLog2e);
       sums[slot] = ((unsigned long long)__float_as_uint(M) << 32) | __float_as_uint(sum);
     }
-    for (int i = threadIdx.x; i < n; i += kThreads) out[i] = 0ull;
     __syncthreads();
-    for (int i = threadIdx.x; i < kWarps * n; i += kThreads) {
-      const int w = i / n, j = i - w * n;
-      if (j >= wcount[w]) continue;
-      const unsigned long long key = wbuf[w * kCap + j];
-      int r = j;
-      for (int q = 0; q < kWarps && r < n; ++q) {
-        if (q == w) continue;
-        // entries of the sorted list q that are better
-        int lo = 0, hi = wcount[q];
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (wbuf[q * kCap + mid] > key) lo = mid + 1; else hi = mid;
-        }
-        r += lo;
+    float bound = red_b[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) bound = fminf(bound, red_b[w]);
+    for (int i = threadIdx.x; i < n; i += kThreads) out[i] = 0ull;
+    for (int c = 0; c < cell; ++c)
+      if (cells[c * kThreads + threadIdx.x] >= bound) {
+        const int at = atomicAdd(&n_hits, 1);
+        if (at < kThreads) hits[at] = c << 8 | (int)threadIdx.x;
       }
-      if (r < n) out[r] = key;
+    __syncthreads();
+    const int hit_n = n_hits;
+    if (hit_n <= kThreads) {
+      // A warp per cell, a lane per element.
+#pragma unroll 2
+      for (int i = warp; i < hit_n; i += kWarps) {
+        const int c = hits[i] >> 8, th = hits[i] & 255, tw = th >> 5;
+        const int tw0 = v0 + (int)((long long)(v1 - v0) * tw / kWarps);
+        const int tw1 = v0 + (int)((long long)(v1 - v0) * (tw + 1) / kWarps);
+        for (int b = 0; b < per_cell; ++b) {
+          const int u = lane / VEC, v = tw0 + (c * per_cell + b) * 32 * kU + u * 32 + (th & 31);
+          const long long idx = (long long)v * VEC - h + lane % VEC;
+          float f = kNegInf;
+          const bool in = lane < kU * VEC && v < tw1 && idx >= 0 && idx < V;
+          if (in) f = to_f32(x[idx]);
+          const bool pass = in && f >= bound;
+          const unsigned vote = __ballot_sync(0xffffffffu, pass);
+          if (!vote) continue;
+          int at = 0;
+          if (lane == 0) at = atomicAdd(&survivors, __popc(vote));
+          at = __shfl_sync(0xffffffffu, at, 0) + __popc(vote & ((1u << lane) - 1u));
+          if (pass && at < kThreads) wbuf[at] = make_key(f, (uint32_t)idx);
+        }
+      }
     }
     __syncthreads();
+    if (hit_n <= kThreads && survivors <= kThreads) {   // all pairs: a thread ranks one survivor
+      const int total = survivors;
+      if ((int)threadIdx.x < total) {
+        const unsigned long long key = wbuf[threadIdx.x];
+        int r = 0;
+#pragma unroll 4
+        for (int i = 0; i < total; ++i) r += wbuf[i] > key ? 1 : 0;
+        if (r < n) out[r] = key;
+      }
+      __syncthreads();
+      continue;
+    }
+    // Very many equal logits: sorted lists.
+    // Read the cells that reach the bound again, in the order of their indices.
+    WarpTop top;
+    top.buf = wbuf + warp * kCap;
+    top.n = n;
+    top.count = 0;
+    top.tau = kNegInf;
+    top.full = false;
+    for (int c = 0; c < cell; ++c) {
+      const float cm = cells[c * kThreads + threadIdx.x];
+      if (!__any_sync(0xffffffffu, cm >= bound && (!top.full || cm > top.tau))) continue;
+      const int end = min(w1, w0 + (c + 1) * per_cell * 32 * kU);
+      for (int base = w0 + c * per_cell * 32 * kU; base < end; base += 32 * kU) {
+        uint4 raw[kU];
+        load(base, raw);
+        const uint32_t* wd = reinterpret_cast<const uint32_t*>(raw);
+        const bool strict = top.full && top.tau >= bound;
+        const float lo = top.full ? fmaxf(top.tau, bound) : bound;
+        uint32_t mask = 0;
+#pragma unroll
+        for (int i = 0; i < kU * VEC; ++i) {
+          const float f = Word<T>::get(wd[i / WN], i % WN);
+          mask |= (strict ? f > lo : f >= lo) ? 1u << i : 0u;
+        }
+        while (true) {
+          bool pass = mask != 0;
+          if (!__any_sync(0xffffffffu, pass)) break;
+          const int bit = pass ? __ffs(mask) - 1 : 0;
+          mask &= mask - 1;
+          const int v = base + (bit / VEC) * 32 + lane;
+          const long long idx = (long long)v * VEC - h + bit % VEC;
+          pass = pass && v < w1 && idx >= 0 && idx < V;
+          const float f = pass ? to_f32(x[idx]) : 0.f;
+          unsigned vote = __ballot_sync(0xffffffffu, pass);
+          if (top.count + __popc(vote) > kCap) {
+            // Elements of this tile are in no order: equal values still compete by index.
+            top_compact(top, lane);
+            pass = pass && (!top.full || f >= top.tau);
+            vote = __ballot_sync(0xffffffffu, pass);
+          }
+          if (pass)
+            top.buf[top.count + __popc(vote & ((1u << lane) - 1u))] = make_key(f, (uint32_t)idx);
+          top.count += __popc(vote);
+        }
+      }
+    }
+    top_compact(top, lane);
+    if (lane == 0) wcount[warp] = top.count;
+    __syncthreads();
+    merge_warps(wbuf, wcount, n, tmp, tlen, out);
   }
   cluster_sync_all();   // every list is written
-  if (rank == 0) {
-    // All lists and sums, from the CTA that made them.
-    for (int i = threadIdx.x; i < tasks * n; i += kThreads) {
-      const int t = i / n, j = i - t * n;
-      all[i] = ld_dsmem_u64(dsmem_addr(smem_u32(lists + (size_t)(t / (int)C) * n + j),
-                                       (uint32_t)(t % (int)C)));
-    }
-    for (int k = threadIdx.x; k < K; k += kThreads) {
-      const long long gk = (long long)g * K + k;
-      const float b = p.beam_scores[gk];
-      double M = -INFINITY, sum = 0.0;
-      for (int sp = 0; sp < S; ++sp) {
-        const int t = k * S + sp;
-        const unsigned long long u =
-            ld_dsmem_u64(dsmem_addr(smem_u32(sums + t / (int)C), (uint32_t)(t % (int)C)));
-        const double mt = (double)__uint_as_float((uint32_t)(u >> 32));
-        const double st = (double)__uint_as_float((uint32_t)u);
-        if (mt > M) {
-          sum = (isinf(M) ? sum : sum * exp(M - mt)) + st;
-          M = mt;
-        } else {
-          sum += isinf(mt) ? st : st * exp(mt - M);
-        }
-      }
-      const double lse = M + log(sum);
-      const bool fin = p.finished && p.finished[gk];
-      row_b[k] = (double)b;
-      row_lse[k] = lse;
-      row_kind[k] = !isfinite(b) ? 1 : fin ? 2 : isfinite(lse) ? 0 : 1;
+  if (rank == 0) {      // all lists and sums, from the CTA that made them
+    for (int i = threadIdx.x; i < tasks * (n + 1); i += kThreads) {
+      const int t = i / (n + 1), j = i - t * (n + 1);
+      const unsigned long long* from = j < n ? lists + (size_t)(t / (int)C) * n + j : sums + t / (int)C;
+      const unsigned long long v = ld_dsmem_u64(dsmem_addr(smem_u32(from), (uint32_t)(t % (int)C)));
+      if (j < n) all[(size_t)t * n + j] = v; else all_sums[t] = v;
     }
   }
   cluster_sync_all();   // the peers' shared memory has been read
   if (rank != 0) return;
-  __syncthreads();
-  const int per_row = S * n;
-  // Rows without usable scores offer their lowest tokens at -inf; finished rows eos first.
-  for (int k = 0; k < K; ++k) {
-    if (row_kind[k] == 0) continue;
-    for (int i = threadIdx.x; i < per_row; i += kThreads) {
-      unsigned long long key = 0ull;
-      if (i < n) {
-        if (row_kind[k] == 1) {
-          if (i < V) key = make_key(kNegInf, (uint32_t)i);
-        } else if (i == 0) {
-          key = make_key(0.f, (uint32_t)p.eos);
-        } else {
-          const int tok = i - 1 < p.eos ? i - 1 : i;
-          if (tok < V) key = make_key(kNegInf, (uint32_t)tok);
-        }
-      }
-      all[(size_t)k * per_row + i] = key;
+  for (int k = threadIdx.x; k < K; k += kThreads) {
+    const long long gk = (long long)g * K + k;
+    const float b = p.beam_scores[gk];
+    float M = kNegInf;
+    double sum = 0.0;
+    for (int sp = 0; sp < S; ++sp)
+      M = fmaxf(M, __uint_as_float((uint32_t)(all_sums[k * S + sp] >> 32)));
+    for (int sp = 0; sp < S; ++sp) {
+      const unsigned long long u = all_sums[k * S + sp];
+      const float mt = __uint_as_float((uint32_t)(u >> 32)), st = __uint_as_float((uint32_t)u);
+      sum += mt == kNegInf ? st : (double)(st * ex2((mt - M) * kLog2e));
     }
+    const double lse = (double)M + log(sum);
+    const bool fin = p.finished && p.finished[gk];
+    row_b[k] = (double)b;
+    row_lse[k] = lse;
+    row_kind[k] = !isfinite(b) ? 1 : fin ? 2 : isfinite(lse) ? 0 : 1;
+  }
+  if (threadIdx.x == 0) survivors = 0;
+  __syncthreads();
+  // The candidates.  Rows without usable scores offer their lowest tokens at -inf, finished
+  // rows eos and then those; both in their first list.
+  for (int i = threadIdx.x; i < tasks * n; i += kThreads) {
+    const int t = i / n, j = i - t * n, k = t / S;
+    Cand c;
+    double sc = -INFINITY;
+    c.tie = (1ull << 62) + i;            // no entry
+    const int kind = row_kind[k];
+    if (kind == 0) {
+      const unsigned long long key = all[i];
+      if (key != 0ull) {
+        sc = row_b[k] + ((double)key_value(key) - row_lse[k]);
+        c.tie = (unsigned long long)k << 32 | key_index(key);
+      }
+    } else if (t == k * S) {
+      int tok = j;
+      if (kind == 2) {
+        tok = j == 0 ? p.eos : j - 1 < p.eos ? j - 1 : j;
+        if (j == 0) sc = row_b[k];
+      }
+      if (tok < V) c.tie = (unsigned long long)k << 32 | (uint32_t)tok;
+    }
+    c.score = score_bits(sc);
+    cand[i] = c;
   }
   __syncthreads();
-  auto score_of = [&](int k, unsigned long long key) -> double {
-    const float v = key_value(key);
-    if (row_kind[k] == 1) return -INFINITY;
-    if (row_kind[k] == 2) return v == 0.f ? row_b[k] : -INFINITY;
-    return row_b[k] + ((double)v - row_lse[k]);
-  };
-  // Rank of every candidate: how many of the sorted lists' entries are better.
-  for (int i = threadIdx.x; i < tasks * n; i += kThreads) {
-    const unsigned long long key = all[i];
-    if (key == 0ull) continue;
-    const int t = i / n, j = i - t * n, k = t / S;
-    const double sc = score_of(k, key);
-    const long long flat = (long long)k * V + key_index(key);
-    int r = j;
-    for (int q = 0; q < tasks && r < n; ++q) {
-      if (q == t) continue;
-      const int kq = q / S;
-      const unsigned long long* L = all + (size_t)q * n;
-      int lo = 0, hi = n;
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        const unsigned long long o = L[mid];
-        bool better = false;
-        if (o != 0ull) {
-          if (kq == k) {
-            better = o > key;
-          } else {
-            const double so = score_of(kq, o);
-            better = so > sc || (so == sc && (long long)kq * V + key_index(o) < flat);
+  // Every list has n entries, so the best of their last ones bounds the n-th best.
+  unsigned long long bound = 0;
+#pragma unroll 4
+  for (int t = 0; t < tasks; ++t) {
+    const unsigned long long o = cand[(size_t)t * n + n - 1].score;
+    bound = o > bound ? o : bound;
+  }
+  for (int i = threadIdx.x; i < tasks * n; i += kThreads)
+    if (cand[i].score >= bound) {
+      const int at = atomicAdd(&survivors, 1);
+      if (at < kThreads) half[at] = cand[i];
+    }
+  __syncthreads();
+  Cand* src = cand;
+  if (survivors <= kThreads) {
+    // Eight lanes compare a survivor with all others.
+    const int total = survivors;
+    for (int i = threadIdx.x >> 3; i < (total + 3) / 4 * 4; i += kThreads / 8) {
+      const Cand c = half[min(i, total - 1)];
+      int r = 0;
+#pragma unroll 2
+      for (int o = lane & 7; o < total; o += 8) r += better(half[o], c) ? 1 : 0;
+      r += __shfl_xor_sync(0xffffffffu, r, 1);
+      r += __shfl_xor_sync(0xffffffffu, r, 2);
+      r += __shfl_xor_sync(0xffffffffu, r, 4);
+      if ((lane & 7) == 0 && i < total && r < n) cand[r] = c;
+    }
+    __syncthreads();
+  } else {
+    // Merge the tasks' lists in pairs until one is left.
+    Cand* dst = half;
+    for (int left = tasks; left > 1; left = (left + 1) / 2) {
+      for (int i = threadIdx.x; i < left * n; i += kThreads) {
+        const int w = i / n, j = i - w * n;
+        const Cand c = src[i];
+        int r = j;
+        if ((w ^ 1) < left) {
+          const Cand* o = src + (size_t)(w ^ 1) * n;
+          int lo = 0, hi = n;
+          while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (better(o[mid], c)) lo = mid + 1; else hi = mid;
           }
+          r += lo;
         }
-        if (better) lo = mid + 1; else hi = mid;
+        if (r < n) dst[(size_t)(w >> 1) * n + r] = c;
       }
-      r += lo;
+      __syncthreads();
+      Cand* x = src;
+      src = dst;
+      dst = x;
     }
-    if (r < n) {
-      const long long o = (long long)g * n + r;
-      p.out_scores[o] = (float)sc;
-      p.out_beams[o] = k;
-      p.out_tokens[o] = (int64_t)key_index(key);
-    }
+  }
+  for (int r = threadIdx.x; r < n; r += kThreads) {
+    const long long o = (long long)g * n + r;
+    const Cand c = src[r];
+    p.out_scores[o] = (float)bits_score(c.score);
+    p.out_beams[o] = (int32_t)(c.tie >> 32);
+    p.out_tokens[o] = (int64_t)(uint32_t)c.tie;
   }
 }
 
@@ -511,14 +765,13 @@ template <typename T>
 static cudaError_t launch_select_t(const beam::SelectParams& p0, int G, cudaStream_t stream) {
   beam::SelectParams p = p0;
   auto kern = beam::beam_select_kernel<T>;
-  // CTAs per prompt: 16 while that leaves SMs idle, else 8 (the portable size).
-  const int C = G <= 16 ? 16 : 8;
+  // CTAs per prompt: as many as run at once, two per SM (64 prompts of 8 beams: 4 CTAs each
+  // 41 us, 8 CTAs 44 to 52 us, 16 CTAs 63 us: what a row costs besides its logits).
+  int C = 16;
+  while (C > 1 && (long long)G * C > 2 * 148) C /= 2;
   p.splits = C / p.K > 1 ? C / p.K : 1;
   const int tasks = p.K * p.splits, per = (tasks + C - 1) / C;
-  const size_t smem = sizeof(unsigned long long) *
-                          ((size_t)beam::kWarps * beam::kCap + (size_t)per * p.n + per +
-                           (size_t)tasks * p.n) +
-                      (size_t)p.K * (2 * sizeof(double) + sizeof(int));
+  const size_t smem = beam::select_smem(p.K, p.n, tasks, per);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e == cudaSuccess && C > 8)
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
