@@ -772,9 +772,7 @@ static cudaError_t launch_select_t(const beam::SelectParams& p0, int G, cudaStre
   p.splits = C / p.K > 1 ? C / p.K : 1;
   const int tasks = p.K * p.splits, per = (tasks + C - 1) / C;
   const size_t smem = beam::select_smem(p.K, p.n, tasks, per);
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e == cudaSuccess && C > 8)
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  cudaError_t e = allow_shared_memory<beam::beam_select_kernel<T>>(true);
   if (e != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -11,6 +11,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/llm_cuda_b200.h"
 
 namespace llmc {
@@ -287,6 +289,29 @@ __device__ __forceinline__ void rope_pair2(uint32_t& x1, uint32_t& x2, uint32_t 
   }
   x1 = *reinterpret_cast<uint32_t*>(o1);
   x2 = *reinterpret_cast<uint32_t*>(o2);
+}
+
+// Gives a kernel all the dynamic shared memory that its static use leaves (and, if asked,
+// clusters of 16) on the current device.  Once per device: the calls cost half a microsecond
+// of a launch's host time.
+template <auto Kern>
+inline cudaError_t allow_shared_memory(bool big_cluster = false) {
+  static std::atomic<unsigned long long> done{0};
+  int dev = 0, most = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  cudaFuncAttributes fa;
+  e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, Kern);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             most - (int)fa.sharedSizeBytes);
+  if (e == cudaSuccess && big_cluster)
+    e = cudaFuncSetAttribute(Kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 }  // namespace llmc

@@ -282,34 +282,26 @@ size_t shared_prefix_workspace_bytes(int B, int Hq, int Hkv, int d, int P, int G
   return tc > gen ? tc : gen;
 }
 
-template <typename... KArgs, typename... Args>
-static cudaError_t launch_chained(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem,
-                                  int cluster, bool early, cudaStream_t stream, Args... args) {
+// Launches with programmatic stream serialization: the kernel's start may overlap its
+// predecessor, whose results it reads only after griddepcontrol.wait.
+template <auto Kern, typename... Args>
+static cudaError_t launch_chained(dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                                  const Args&... args) {
   if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem);
+    cudaError_t e = allow_shared_memory<Kern>();
     if (e != cudaSuccess) return e;
   }
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (early) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n++].val.programmaticStreamSerializationAllowed = 1;
-  }
-  if (cluster > 1) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = cluster;
-    attr[n].val.clusterDim.y = 1;
-    attr[n++].val.clusterDim.z = 1;
-  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = n;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, Kern, args...);
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
@@ -327,13 +319,13 @@ static cudaError_t launch_generic(prefix::Params p, float* ws, std::string* err,
     *err = "more than 65535 row tiles (groups x max_group, sequences) for this shape";
     return cudaErrorInvalidConfiguration;
   }
-  cudaError_t e = launch_chained(gen::units_kernel<T>, dim3(p.nsplit, (unsigned)units, p.Hkv),
-                                 dim3(gen::kThreads), gen::smem_bytes(p.d), 1, true, stream, p,
-                                 group_tiles, seq_tiles);
+  cudaError_t e = launch_chained<gen::units_kernel<T>>(
+      dim3(p.nsplit, (unsigned)units, p.Hkv), dim3(gen::kThreads), gen::smem_bytes(p.d), stream, p,
+      group_tiles, seq_tiles);
   if (e != cudaSuccess) return e;
   const long long rows = (long long)p.B * p.Hq;
-  return launch_chained(gen::join_kernel<T>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, 1,
-                        true, stream, p);
+  return launch_chained<gen::join_kernel<T>>(dim3((unsigned)((rows + 7) / 8)), dim3(256), 0,
+                                             stream, p);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -435,19 +427,19 @@ static cudaError_t launch_tc(const prefix::Params& p0, void* ws, int dtype, std:
   const size_t tables = tc::Tables::ints(p.G, p.B) * sizeof(int);
   cudaError_t e;
   if (fixed + tables > (size_t)di.smem) {
-    e = launch_chained(tc::tables_kernel, dim3(1), dim3(1024), 0, 1, true, stream, tp);
+    e = launch_chained<tc::tables_kernel>(dim3(1), dim3(1024), 0, stream, tp);
     if (e != cudaSuccess) return e;
-    e = launch_chained(tc::parts_kernel<D, T, true>, dim3(di.sms), dim3(tc::kThreads), fixed, 1,
-                       true, stream, mk, mv, mq, mq1, tp);
+    e = launch_chained<tc::parts_kernel<D, T, true>>(dim3(di.sms), dim3(tc::kThreads), fixed,
+                                                     stream, mk, mv, mq, mq1, tp);
   } else {
-    e = launch_chained(tc::parts_kernel<D, T, false>, dim3(di.sms), dim3(tc::kThreads),
-                       fixed + tables, 1, true, stream, mk, mv, mq, mq1, tp);
+    e = launch_chained<tc::parts_kernel<D, T, false>>(dim3(di.sms), dim3(tc::kThreads),
+                                                      fixed + tables, stream, mk, mv, mq, mq1, tp);
   }
   if (e != cudaSuccess) return e;
   const long long out_rows = (long long)p.B * p.Hq;
   constexpr int per = 256 / (D / 4);
-  return launch_chained(tc::join_kernel<D, T>, dim3((unsigned)((out_rows + per - 1) / per)),
-                        dim3(256), 0, 1, true, stream, tp);
+  return launch_chained<tc::join_kernel<D, T>>(dim3((unsigned)((out_rows + per - 1) / per)),
+                                               dim3(256), 0, stream, tp);
 }
 
 cudaError_t launch_shared_prefix_decode(const void* q, const void* kp, const void* vp,

@@ -82,11 +82,11 @@ def beam_select(
     scores = torch.empty(G, n, dtype=torch.float32, device=dev)
     beams = torch.empty(G, n, dtype=torch.int32, device=dev)
     tokens = torch.empty(G, n, dtype=torch.int64, device=dev)
-    with torch.cuda.device(dev):
+    with N.on_device(dev):
         rc = lib.llmc_beam_select(
             logits.data_ptr(), stride, beam_scores.data_ptr(), N.ptr(finished), scores.data_ptr(),
             beams.data_ptr(), tokens.data_ptr(), G, K, V, n, eos, N.dtype_code(logits.dtype),
-            N.stream_handle(dev))
+            N.raw_stream(dev))
     N.check(rc, "llmc_beam_select")
     return scores, beams, tokens
 
@@ -137,9 +137,9 @@ def beam_reorder(
     parents = parents.contiguous()
     layers, _, num_pages, Hkv, P, d = pools.shape
     st = status if status is not None else default_status(pools.device)
-    with torch.cuda.device(pools.device):
+    with N.on_device(pools.device):
         rc = lib.llmc_beam_reorder(
             pools.data_ptr(), own_table.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
             parents.data_ptr(), st.data_ptr(), G, K, layers, Hkv, d, P, own_table.shape[1],
-            num_pages, pools.element_size(), N.stream_handle(pools.device))
+            num_pages, pools.element_size(), N.raw_stream(pools.device))
     N.check(rc, "llmc_beam_reorder")

@@ -13,6 +13,7 @@ to the tensor type's accuracy, not bit for bit.
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -56,28 +57,34 @@ def shared_prefix_decode(
     lib = N.load()
     if not q.is_cuda:
         raise ValueError("shared_prefix_decode needs CUDA tensors")
-    if q.dim() not in (3, 4) or (q.dim() == 4 and q.shape[2] != 1):
+    dev, dtype, q_shape = q.device, q.dtype, q.shape
+    if len(q_shape) == 4:
+        if q_shape[2] != 1:
+            raise ValueError("q must be [B, Hq, d] or [B, Hq, 1, d]: one query token per sequence")
+        q = q.reshape(q_shape[0], q_shape[1], q_shape[3])
+    elif len(q_shape) != 3:
         raise ValueError("q must be [B, Hq, d] or [B, Hq, 1, d]: one query token per sequence")
-    q_shape = q.shape
-    q3 = q.reshape(q.shape[0], q.shape[1], q.shape[-1]).contiguous()
-    B, Hq, d = q3.shape
-    if key_pages.dim() != 4 or value_pages.shape != key_pages.shape or key_pages.shape[3] != d:
+    q = q.contiguous()
+    B, Hq, d = q.shape
+    pages = key_pages.shape
+    if len(pages) != 4 or value_pages.shape != pages or pages[3] != d:
         raise ValueError("pages must be [num_pages, Hkv, page_size, d] with the head_dim of q")
-    if key_pages.dtype != q.dtype or value_pages.dtype != q.dtype:
+    if key_pages.dtype != dtype or value_pages.dtype != dtype:
         raise ValueError("q and pages must share a dtype")
-    if key_pages.device != q.device or value_pages.device != q.device:
+    if key_pages.device != dev or value_pages.device != dev:
         raise ValueError("q and pages must be on one device")
     if not (key_pages.is_contiguous() and value_pages.is_contiguous()):
         raise ValueError("pages must be contiguous")
-    num_pages, Hkv, P, _ = key_pages.shape
+    num_pages, Hkv, P, _ = pages
     if Hq % Hkv:
         raise ValueError("n_heads must be a multiple of n_kv_heads")
-    _check_index(block_table, "block_table", 2, q.device)
-    _check_index(seq_lens, "seq_lens", 1, q.device)
-    _check_index(group_starts, "group_starts", 1, q.device)
-    _check_index(shared_lens, "shared_lens", 1, q.device)
+    _check_index(block_table, "block_table", 2, dev)
+    _check_index(seq_lens, "seq_lens", 1, dev)
+    _check_index(group_starts, "group_starts", 1, dev)
+    _check_index(shared_lens, "shared_lens", 1, dev)
     G = shared_lens.shape[0]
-    if block_table.shape[0] != B or seq_lens.shape[0] != B:
+    rows, max_pages = block_table.shape
+    if rows != B or seq_lens.shape[0] != B:
         raise ValueError("block_table and seq_lens must have one row per sequence")
     if group_starts.shape[0] != G + 1:
         raise ValueError("group_starts must have one entry more than shared_lens")
@@ -86,25 +93,31 @@ def shared_prefix_decode(
         raise ValueError("max_group must be positive")
     max_group = max(1, min(max_group, B))
     if out is None:
-        out = torch.empty_like(q3)
-    elif out.shape not in (q3.shape, q_shape) or out.dtype != q.dtype or \
-            out.device != q.device or not out.is_contiguous():
+        out = torch.empty(q_shape, dtype=dtype, device=dev)
+    elif out.shape not in (q.shape, q_shape) or out.dtype != dtype or out.device != dev or \
+            not out.is_contiguous():
         raise ValueError("out must be contiguous and match q")
+    elif out.shape != q_shape:
+        out = out.view(q_shape)
     if B == 0:
-        return out.view(q_shape)
-    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    dt = N.dtype_code(q.dtype)
-    st = status if status is not None else default_status(q.device)
-    with torch.cuda.device(q.device):
-        nbytes = lib.llmc_shared_prefix_workspace_bytes(B, Hq, Hkv, d, P, G, max_group, dt)
+        return out
+    dt = N.dtype_code(dtype)
+    st = status if status is not None else default_status(dev)
+    with N.on_device(dev):
         # From the caching allocator, per call: ordered with the stream, private to a graph
         # that captures it, never shared by two calls in flight.
-        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+        nbytes = _workspace_bytes(dev.index, B, Hq, Hkv, d, P, G, max_group, dt)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         rc = lib.llmc_shared_prefix_decode(
-            q3.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), block_table.data_ptr(),
+            q.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), block_table.data_ptr(),
             seq_lens.data_ptr(), group_starts.data_ptr(), shared_lens.data_ptr(), out.data_ptr(),
-            ws.data_ptr(), ws.numel(), st.data_ptr(), B, Hq, Hkv, d, P, block_table.shape[1],
-            num_pages, G, max_group, scale, dt,
-            N.LLMC_DECODE_FORCE_GENERIC if force_generic else 0, N.stream_handle(q.device))
+            ws.data_ptr(), nbytes, st.data_ptr(), B, Hq, Hkv, d, P, max_pages, num_pages, G,
+            max_group, 1.0 / math.sqrt(d) if scale is None else float(scale), dt,
+            N.LLMC_DECODE_FORCE_GENERIC if force_generic else 0, N.raw_stream(dev))
     N.check(rc, "llmc_shared_prefix_decode")
-    return out.view(q_shape)
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device_index: int, *sizes: int) -> int:
+    return max(16, N.load().llmc_shared_prefix_workspace_bytes(*sizes))
