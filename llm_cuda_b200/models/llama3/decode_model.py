@@ -35,8 +35,9 @@ from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 
+from ...kernels.beam import beam_select
 from ...kernels.step_ops import add_rmsnorm, argmax_rows, decode_gemm, swiglu
-from .kv_cache import PagedKVCache, make_block_table
+from .kv_cache import BeamKVCache, PagedKVCache, make_block_table
 from .rotary import RopeTable
 
 
@@ -370,6 +371,51 @@ class Llama3DecodeModel:
         logits = self._lm_head(h[:, 0])
         mark("lm_head")
         return logits
+
+    def make_beam_cache(self, prompt_lens: list[int], beams: int, max_seq_len: int,
+                        page_size: int = 16, shuffle_seed: int | None = None) -> BeamKVCache:
+        """Cache of ``beams`` beams per prompt for this rank's KV heads."""
+        gen = None if shuffle_seed is None else torch.Generator().manual_seed(shuffle_seed)
+        return BeamKVCache(self.cfg.num_hidden_layers, self.hkv, self.cfg.head_dim, max_seq_len,
+                           page_size, self.device, self.dtype, prompt_lens, beams, generator=gen)
+
+    def beam_search(self, ids: torch.Tensor, beams: int, max_new_tokens: int,
+                    eos_token_id: int | None = None, page_size: int = 16,
+                    shuffle_seed: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The best ``beams`` continuations of each prompt ``ids [G, S]`` by their summed
+        log-probabilities, best first: ``(tokens [G, beams, max_new_tokens], scores [G, beams])``.
+
+        The reference generates greedily (``model.py:178-218``).  A beam that has produced
+        ``eos_token_id`` keeps its score and repeats it.  Per step: one decode step over the
+        beams (the prompt's pages read once per prompt), one selection, one reordering of the
+        cache; nothing waits for the host.
+        """
+        G, S = ids.shape
+        if max_new_tokens < 1:
+            raise ValueError("max_new_tokens must be > 0")
+        if not 1 <= beams <= self.cfg.vocab_size:
+            raise ValueError("beams must be 1 to the vocabulary's size")
+        cache = self.make_beam_cache([S] * G, beams, S + max_new_tokens, page_size, shuffle_seed)
+        leaders = cache.leaders()
+        logits = self.prefill(ids, leaders)
+        cache.fork()
+        zero = torch.zeros(G, 1, dtype=torch.float32, device=self.device)
+        scores, _, tokens = beam_select(logits, zero, num_out=beams)
+        out = torch.empty(G, beams, max_new_tokens, dtype=torch.int64, device=self.device)
+        out[..., 0] = tokens
+        finished = None if eos_token_id is None else tokens == eos_token_id
+        for step in range(1, max_new_tokens):
+            logits = self.decode_step(tokens.view(-1), cache)
+            scores, parents, tokens = beam_select(logits, scores, num_out=beams,
+                                                  finished=finished, eos_token_id=eos_token_id)
+            cache.reorder(parents)
+            rows = parents.long()
+            out = out.gather(1, rows[..., None].expand_as(out))
+            out[..., step] = tokens
+            if finished is not None:
+                finished = finished.gather(1, rows) | (tokens == eos_token_id)
+        self.check_status(cache)
+        return out, scores
 
     def bytes_per_step(self, cache: PagedKVCache) -> tuple[int, int]:
         """(weight bytes, KV bytes) this rank reads in one decode step at the current

@@ -22,6 +22,10 @@ kv_cache.py:43-44,55-57):
 
 ``get_kv()`` still returns the gathered ``[B, Hkv, len, d]`` tensors for
 compatibility; the decode path never calls it.
+
+``BeamKVCache`` holds the beams of several prompts: the pages of a prompt are shared by
+its beams, attention reads them once for all of them, and ``reorder`` lets every beam
+continue from its parent.
 """
 
 from __future__ import annotations
@@ -36,7 +40,9 @@ from ...kernels.decode_attention import (
     paged_decode_attention,
     rope_append_decode,
 )
+from ...kernels.beam import beam_reorder
 from ...kernels.rope import rope_append
+from ...kernels.shared_prefix import shared_prefix_decode
 from .rotary import RopeTable
 
 
@@ -62,6 +68,43 @@ def make_block_table(batch_size: int, pages_per_seq, num_pages: int, max_pages: 
     return bt.to(device) if device is not None else bt
 
 
+def make_beam_table(prompt_lens: list[int], beams: int, page_size: int, max_pages: int,
+                    generator: torch.Generator | None = None) -> tuple[torch.Tensor, int]:
+    """``(own_table, num_pages)`` for ``beams`` beams of each prompt: the full pages of a
+    prompt are named by all its beams, every later logical page is a beam's own.  Pages in
+    random order when a ``generator`` is given."""
+    if beams < 1:
+        raise ValueError("beams must be > 0")
+    rows, n = [], 0
+    for length in prompt_lens:
+        full = length // page_size
+        if length < 0 or full > max_pages:
+            raise ValueError("a prompt needs more pages than max_pages")
+        common = torch.arange(n, n + full)
+        n += full
+        own = torch.arange(n, n + beams * (max_pages - full)).view(beams, -1)
+        n += own.numel()
+        rows.append(torch.cat([common.expand(beams, -1), own], 1))
+    table = torch.cat(rows)
+    if generator is not None:
+        table = torch.randperm(n, generator=generator)[table]
+    return table.to(torch.int32), max(n, 1)
+
+
+class SharedPrefix:
+    """Which sequences of a batch hold the same first tokens (see ``shared_prefix_decode``)."""
+
+    def __init__(self, group_starts: list[int], shared_lens: list[int], device):
+        if len(group_starts) != len(shared_lens) + 1:
+            raise ValueError("group_starts needs one entry more than shared_lens")
+        sizes = [b - a for a, b in zip(group_starts, group_starts[1:])]
+        if any(x < 0 for x in sizes) or (group_starts and group_starts[0] < 0):
+            raise ValueError("groups must be ascending ranges of the batch")
+        self.group_starts = torch.tensor(group_starts, dtype=torch.int32, device=device)
+        self.shared_lens = torch.tensor(shared_lens, dtype=torch.int32, device=device)
+        self.max_group = max(sizes, default=1) or 1
+
+
 class PagedKVLayerCache:
     def __init__(
         self,
@@ -76,7 +119,13 @@ class PagedKVLayerCache:
         block_table: torch.Tensor | None = None,
         workspace: DecodeWorkspace | None = None,
         status: torch.Tensor | None = None,
+        key_pages: torch.Tensor | None = None,
+        value_pages: torch.Tensor | None = None,
+        shared: SharedPrefix | None = None,
     ):
+        """``key_pages``/``value_pages``: pools that exist already (``[num_pages, Hkv, P, d]``,
+        contiguous).  ``shared``: the batch's common prefixes; decode then reads them once
+        for all sequences of a group."""
         if page_size <= 0:
             raise ValueError("page_size must be > 0")
         if max_seq_len <= 0:
@@ -104,9 +153,18 @@ class PagedKVLayerCache:
                 num_pages = int(block_table.max().item()) + 1
         self.num_pages = num_pages
         self.block_table = block_table.to(device=device, dtype=torch.int32).contiguous()
-        self.key_pages = torch.empty(num_pages, num_kv_heads, page_size, head_dim, device=device,
-                                     dtype=dtype)
-        self.value_pages = torch.empty_like(self.key_pages)
+        if (key_pages is None) != (value_pages is None):
+            raise ValueError("key_pages and value_pages go together")
+        if key_pages is None:
+            key_pages = torch.empty(num_pages, num_kv_heads, page_size, head_dim, device=device,
+                                    dtype=dtype)
+            value_pages = torch.empty_like(key_pages)
+        elif any(t.shape != (num_pages, num_kv_heads, page_size, head_dim) or t.dtype != dtype
+                 or not t.is_contiguous() for t in (key_pages, value_pages)):
+            raise ValueError("pools must be contiguous [num_pages, Hkv, page_size, d] in dtype")
+        self.key_pages = key_pages
+        self.value_pages = value_pages
+        self.shared = shared
         self.seq_lens = torch.zeros(batch_size, dtype=torch.int32, device=device)
         self.host_lengths = [0] * batch_size
         self.workspace = workspace if workspace is not None else DecodeWorkspace(device)
@@ -162,10 +220,15 @@ class PagedKVLayerCache:
         """The whole decode-attention step of the new token: RoPE on q/k, page append
         and paged attention over the grown context, fused into one decode kernel (plus
         the merge).  Same results as ``append_rotary`` followed by ``decode``.
-        ``early_tables``: see ``kernels.decode_attention.rope_append_decode``."""
+        ``early_tables``: see ``kernels.decode_attention.rope_append_decode``.  With shared
+        prefixes: RoPE and the append in one launch, then ``shared_prefix_decode``."""
         seq = self._check_kv(k, v)
         if seq != 1:
             raise ValueError("rope_append_decode takes one new token per sequence")
+        if self.shared is not None:
+            q_rot = self.append_rotary(q, k, v, rope,
+                                       q_out=q_out if q_out is None else q_out.view(q.shape))
+            return self.decode(q_rot, out=out, partition_tokens=partition_tokens)
         res = rope_append_decode(q, k, v, self.key_pages, self.value_pages, self.block_table,
                                  self.seq_lens, rope.cos, rope.sin, host_lens=self.host_lengths,
                                  partition_tokens=partition_tokens, out=out, q_out=q_out,
@@ -181,6 +244,13 @@ class PagedKVLayerCache:
     def decode(self, q: torch.Tensor, out: torch.Tensor | None = None,
                partition_tokens: int | None = None) -> torch.Tensor:
         """Paged decode attention of ``q [B, Hq, 1, d]`` against this cache."""
+        if self.shared is not None:
+            if partition_tokens:
+                raise ValueError("decode over shared prefixes takes no partition_tokens")
+            return shared_prefix_decode(q, self.key_pages, self.value_pages, self.block_table,
+                                        self.seq_lens, self.shared.group_starts,
+                                        self.shared.shared_lens, max_group=self.shared.max_group,
+                                        out=out, status=self.status)
         return paged_decode_attention(q, self, out=out, partition_tokens=partition_tokens)
 
     def get_kv(self) -> tuple[torch.Tensor, torch.Tensor]:
@@ -255,6 +325,78 @@ class PagedKVCache:
 
     def check_status(self) -> None:
         self.layer_caches[0].check_status()
+
+
+class BeamKVCache(PagedKVCache):
+    """The paged cache of a beam search: ``beams`` beams of each prompt, in the order
+    ``prompt * beams + beam``.
+
+    The pools of all layers are one tensor, ``pools [layers, 2, num_pages, Hkv, P, d]``.
+    ``own_table`` names the pages that each beam writes (a prompt's full pages, then the
+    beam's own), ``block_table`` those that it reads; reordering moves entries of the
+    latter and copies only the page in progress.  The layers attend with the prompt as
+    shared prefix.  Usage: prefill ``leaders()`` with one sequence per prompt, ``fork()``,
+    then per step a decode, a selection and ``reorder(parents)``.
+    """
+
+    def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, max_seq_len: int,
+                 page_size: int, device, dtype: torch.dtype, prompt_lens: list[int], beams: int,
+                 generator: torch.Generator | None = None):
+        if not prompt_lens:
+            raise ValueError("prompt_lens must not be empty")
+        if max(prompt_lens) > max_seq_len or min(prompt_lens) < 1:
+            raise ValueError("prompts must have 1 to max_seq_len tokens")
+        device = torch.device(device)
+        self.prompt_lens, self.beams = list(prompt_lens), beams
+        max_pages = math.ceil(max_seq_len / page_size)
+        own, num_pages = make_beam_table(prompt_lens, beams, page_size, max_pages, generator)
+        self.own_table = own.to(device)
+        self.block_table = self.own_table.clone()
+        self.pools = torch.empty(num_layers, 2, num_pages, num_kv_heads, page_size, head_dim,
+                                 device=device, dtype=dtype)
+        self.shared = SharedPrefix([g * beams for g in range(len(prompt_lens) + 1)], prompt_lens,
+                                   device)
+        ws = DecodeWorkspace(device)
+        status = torch.zeros(1, dtype=torch.int32, device=device)
+        common = dict(num_kv_heads=num_kv_heads, head_dim=head_dim, max_seq_len=max_seq_len,
+                      page_size=page_size, device=device, dtype=dtype, num_pages=num_pages,
+                      workspace=ws, status=status)
+        super().__init__([
+            PagedKVLayerCache(**common, batch_size=len(prompt_lens) * beams,
+                              block_table=self.block_table, key_pages=self.pools[i, 0],
+                              value_pages=self.pools[i, 1], shared=self.shared)
+            for i in range(num_layers)])
+        self._common = common
+
+    def leaders(self) -> PagedKVCache:
+        """The first beam of every prompt as a cache of its own over the same pages (empty):
+        what a prefill fills."""
+        table = self.own_table[::self.beams].contiguous()
+        return PagedKVCache([
+            PagedKVLayerCache(**self._common, batch_size=len(self.prompt_lens), block_table=table,
+                              key_pages=self.pools[i, 0], value_pages=self.pools[i, 1])
+            for i in range(len(self.layer_caches))])
+
+    def fork(self) -> None:
+        """After a prefill of ``leaders()``: every beam holds its prompt."""
+        lens = [n for n in self.prompt_lens for _ in range(self.beams)]
+        device_lens = torch.tensor(lens, dtype=torch.int32, device=self.pools.device)
+        for layer in self.layer_caches:
+            layer.seq_lens.copy_(device_lens)
+            layer.host_lengths = list(lens)
+        self.block_table.copy_(self.own_table)
+        self.reorder(torch.zeros(len(self.prompt_lens), self.beams, dtype=torch.int32,
+                                 device=self.pools.device))
+
+    def reorder(self, parents: torch.Tensor) -> None:
+        """Beam ``i`` of prompt ``g`` continues from beam ``parents[g, i]`` (int32, on the
+        device), in all layers; see ``kernels.beam.beam_reorder``."""
+        beam_reorder(self.pools, self.own_table, self.block_table,
+                     self.layer_caches[0].seq_lens, parents, status=self.layer_caches[0].status)
+
+    def clear(self) -> None:
+        super().clear()
+        self.block_table.copy_(self.own_table)
 
 
 class GraphedDecodeStep:

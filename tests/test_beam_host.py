@@ -84,3 +84,52 @@ def test_python_entry_points_refuse_cpu_tensors():
         beam_select(torch.zeros(2, 10), torch.zeros(1, 2))
     with pytest.raises(ValueError, match="CUDA"):
         beam_reorder(torch.zeros(1, 2, 4, 2, 16, 64), i.view(2, 1), i.view(2, 1), i, i.view(1, 2))
+
+
+def test_beam_table_shares_the_prompts_full_pages():
+    from llm_cuda_b200.models.llama3 import make_beam_table
+
+    table, n = make_beam_table([33, 0, 48], beams=3, page_size=16, max_pages=4)
+    assert table.shape == (9, 4) and n == (2 + 3 * 2) + 3 * 4 + (3 + 3 * 1)
+    assert (table[0:3, :2] == table[0, :2]).all()            # 32 tokens shared
+    assert (table[6:9, :3] == table[6, :3]).all()
+    own = torch.cat([table[0:3, 2:].flatten(), table[3:6].flatten(), table[6:9, 3:].flatten()])
+    names = torch.cat([own, table[0, :2], table[6, :3]]).tolist()
+    assert sorted(names) == list(range(n))                   # every page once
+    shuffled, m = make_beam_table([33, 0, 48], 3, 16, 4, torch.Generator().manual_seed(0))
+    assert m == n and sorted(set(shuffled.flatten().tolist())) == list(range(n))
+    with pytest.raises(ValueError, match="max_pages"):
+        make_beam_table([65], 2, 16, 4 - 1)
+    with pytest.raises(ValueError, match="beams"):
+        make_beam_table([5], 0, 16, 4)
+
+
+def test_beam_cache_layout_and_refusals():
+    from llm_cuda_b200.models.llama3 import BeamKVCache, PagedKVLayerCache, SharedPrefix
+
+    c = BeamKVCache(2, 2, 64, 40, 16, "cpu", torch.bfloat16, [20, 33], beams=4)
+    assert c.pools.shape == (2, 2, 1 + 4 * 2 + 2 + 4 * 1, 2, 16, 64)
+    for i, layer in enumerate(c.layer_caches):
+        assert layer.batch_size == 8
+        assert layer.key_pages.data_ptr() == c.pools[i, 0].data_ptr()
+        assert layer.value_pages.data_ptr() == c.pools[i, 1].data_ptr()
+        assert layer.block_table.data_ptr() == c.block_table.data_ptr()   # one table
+    assert c.shared.max_group == 4 and c.shared.group_starts.tolist() == [0, 4, 8]
+    lead = c.leaders().get_layer(1)
+    assert lead.batch_size == 2 and lead.shared is None
+    assert torch.equal(lead.block_table, c.own_table[::4])
+    assert lead.key_pages.data_ptr() == c.pools[1, 0].data_ptr()
+    with pytest.raises(ValueError, match="prompt"):
+        BeamKVCache(1, 2, 64, 40, 16, "cpu", torch.bfloat16, [41], 2)
+    with pytest.raises(ValueError, match="prompt"):
+        BeamKVCache(1, 2, 64, 40, 16, "cpu", torch.bfloat16, [], 2)
+    with pytest.raises(ValueError, match="ascending"):
+        SharedPrefix([0, 3, 2], [1, 1], "cpu")
+    with pytest.raises(ValueError, match="one entry more"):
+        SharedPrefix([0, 3], [1, 1], "cpu")
+    kv = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="go together"):
+        PagedKVLayerCache(2, 64, 64, 16, "cpu", torch.bfloat16, key_pages=kv)
+    with pytest.raises(ValueError, match="pools must be"):
+        PagedKVLayerCache(2, 64, 64, 16, "cpu", torch.bfloat16, key_pages=kv[:3],
+                          value_pages=kv[:3])
