@@ -13,8 +13,9 @@
 // bf16/fp16 at head size 64 or 128 and pages of 8, 16, 32, 64 or a multiple of 128 tokens
 // run on the tensor cores (shared_prefix_tc.cuh).  The kernels of this file take every
 // other type, head size and page size: shared-prefix rows and own rows alike are cut into
-// units of 16 query rows x a range of tokens, in fp32 on the CUDA cores, with 32 tokens of
-// K and V at a time in shared memory.
+// units of 16 or 64 query rows x a range of tokens, in fp32 on the CUDA cores, with 32
+// tokens of K and V at a time in shared memory.  Bound: the FMA pipes and, as evenly, the
+// shared-memory reads that feed them (4 rows x 2 tokens or 4 rows x 4 columns a thread).
 #include <climits>
 #include <string>
 
@@ -24,152 +25,239 @@ namespace llmc {
 namespace prefix {
 namespace generic {
 
-constexpr int kRows = 16;     // query rows of a unit
 constexpr int kTok = 32;      // tokens per step
-constexpr int kThreads = 256; // 16 threads per row
+constexpr int kThreads = 256; // 16 threads per group of rows
 
-__host__ __device__ inline size_t smem_bytes(int d) {
-  return sizeof(float) * ((size_t)kRows * d + (size_t)kTok * (d + 1) + (size_t)kTok * d +
-                          kRows * (kTok + 1));
+// Shared memory of a unit of 16 * RPT rows: Q, K (rows of dp + 4 floats), V, P.
+__host__ __device__ inline size_t smem_floats(int rpt, int dp) {
+  return (size_t)16 * rpt * (dp + 4) + (size_t)kTok * (dp + 4) + (size_t)kTok * dp +
+         (size_t)16 * rpt * (kTok + 4);
 }
 
-// Partials: part_o [2 * nsplit][B * Hq][d], part_lse [2 * nsplit][B * Hq]; slots below
-// nsplit are the shared part's, the others the own part's.
-// Grid: x = split, y = unit of a KV head, z = KV head.  Units: the tiles of the groups'
-// rows (tiles of a group are sized for max_group), then the tiles of every sequence.
-template <typename T>
+// Where a block works.
+struct Unit {
+  int lo, nrows, row0, table_row, hk, first, last, slot;
+  bool group;
+};
+
+// Attention of rows [row0, row0 + 16 RPT) over tokens [first, last).  Thread (rg, c): rows
+// rg * RPT ..., keys c and c + 16, output columns 4 c + 64 j.
+template <typename T, int NJ, int RPT>
+__device__ __forceinline__ void attend(const Params& p, const Unit& u, float* sm) {
+  constexpr int DP = 64 * NJ, QS = DP + 4, PS = kTok + 4, ROWS = 16 * RPT;
+  float* Qs = sm;                 // [ROWS][QS]
+  float* Ks = Qs + ROWS * QS;     // [32][QS]
+  float* Vs = Ks + kTok * QS;     // [32][DP]
+  float* Ps = Vs + kTok * DP;     // [ROWS][PS]
+  const int d = p.d, tid = threadIdx.x, rg = tid >> 4, c = tid & 15;
+  const T* q = reinterpret_cast<const T*>(p.q);
+  for (int i = tid; i < ROWS * DP; i += kThreads) {
+    const int r = i / DP, col = i - r * DP, row = u.row0 + r;
+    float v = 0.f;
+    if (row < u.nrows && col < d) {
+      const int b = u.lo + row / p.R, h = u.hk * p.R + row % p.R;
+      v = to_f32(q[((long long)b * p.Hq + h) * d + col]) * p.scale_log2;
+    }
+    Qs[r * QS + col] = v;
+  }
+  const T* kp = reinterpret_cast<const T*>(p.k_pages);
+  const T* vp = reinterpret_cast<const T*>(p.v_pages);
+  constexpr int VEC = 16 / sizeof(T);
+  const bool vec = d % VEC == 0 && ((reinterpret_cast<uintptr_t>(kp) |
+                                     reinterpret_cast<uintptr_t>(vp)) & 15) == 0;
+  const float kNegInf = __int_as_float(0xff800000);
+  float m[RPT], l[RPT], acc[RPT][NJ][4];
+#pragma unroll
+  for (int r = 0; r < RPT; ++r) {
+    m[r] = kNegInf;
+    l[r] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[r][j][e] = 0.f;
+  }
+  for (int t0 = u.first; t0 < u.last; t0 += kTok) {
+    const int nt = min(kTok, u.last - t0);
+    __syncthreads();
+    {   // 8 threads per token bring its key and value; columns from d on are zero
+      const int t = tid >> 3, part = tid & 7;
+      const bool have = t < nt;
+      long long base = 0;
+      if (have) {
+        const int tok = t0 + t;
+        base = (((long long)page_of(p, u.table_row, tok) * p.Hkv + u.hk) * p.P + tok % p.P) * d;
+      }
+      if (vec) {
+#pragma unroll
+        for (int i = part * VEC; i < DP; i += 8 * VEC) {
+          uint4 kv = make_uint4(0u, 0u, 0u, 0u), vv = kv;
+          if (have && i < d) {
+            kv = __ldg(reinterpret_cast<const uint4*>(kp + base + i));
+            vv = __ldg(reinterpret_cast<const uint4*>(vp + base + i));
+          }
+          const T* ke = reinterpret_cast<const T*>(&kv);
+          const T* ve = reinterpret_cast<const T*>(&vv);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            Ks[t * QS + i + e] = to_f32(ke[e]);
+            Vs[t * DP + i + e] = to_f32(ve[e]);
+          }
+        }
+      } else {
+        for (int i = part; i < DP; i += 8) {
+          const bool in = have && i < d;
+          Ks[t * QS + i] = in ? to_f32(kp[base + i]) : 0.f;
+          Vs[t * DP + i] = in ? to_f32(vp[base + i]) : 0.f;
+        }
+      }
+    }
+    __syncthreads();
+    float x0[RPT], x1[RPT];
+#pragma unroll
+    for (int r = 0; r < RPT; ++r) x0[r] = x1[r] = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < DP; i += 4) {
+      const float4 k0 = *reinterpret_cast<const float4*>(Ks + c * QS + i);
+      const float4 k1 = *reinterpret_cast<const float4*>(Ks + (c + 16) * QS + i);
+#pragma unroll
+      for (int r = 0; r < RPT; ++r) {
+        const float4 qv = *reinterpret_cast<const float4*>(Qs + (rg * RPT + r) * QS + i);
+        x0[r] = fmaf(qv.x, k0.x, fmaf(qv.y, k0.y, fmaf(qv.z, k0.z, fmaf(qv.w, k0.w, x0[r]))));
+        x1[r] = fmaf(qv.x, k1.x, fmaf(qv.y, k1.y, fmaf(qv.z, k1.z, fmaf(qv.w, k1.w, x1[r]))));
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RPT; ++r) {
+      if (c >= nt) x0[r] = kNegInf;
+      if (c + 16 >= nt) x1[r] = kNegInf;
+      float tm = fmaxf(x0[r], x1[r]);
+#pragma unroll
+      for (int o = 8; o; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
+      const float mn = fmaxf(m[r], tm);
+      const float mu = mn == kNegInf ? 0.f : mn;    // every score -inf: weights 0
+      const float f = exp2f(m[r] - mu);
+      const float p0 = exp2f(x0[r] - mu), p1 = exp2f(x1[r] - mu);
+      float ps = p0 + p1;
+#pragma unroll
+      for (int o = 8; o; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
+      l[r] = l[r] * f + ps;
+      m[r] = mn;
+      Ps[(rg * RPT + r) * PS + c] = p0;
+      Ps[(rg * RPT + r) * PS + c + 16] = p1;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[r][j][e] *= f;
+    }
+    __syncwarp();                                 // a row's threads are in one warp
+    // Weights behind nt are zero and so are V's rows there.
+#pragma unroll 2
+    for (int t = 0; t < kTok; t += 4) {
+      if (t >= nt) break;
+      float4 w[RPT];
+#pragma unroll
+      for (int r = 0; r < RPT; ++r)
+        w[r] = *reinterpret_cast<const float4*>(Ps + (rg * RPT + r) * PS + t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const float4 v = *reinterpret_cast<const float4*>(Vs + (t + e) * DP + 64 * j + 4 * c);
+#pragma unroll
+          for (int r = 0; r < RPT; ++r) {
+            const float pw = e == 0 ? w[r].x : e == 1 ? w[r].y : e == 2 ? w[r].z : w[r].w;
+            acc[r][j][0] = fmaf(pw, v.x, acc[r][j][0]);
+            acc[r][j][1] = fmaf(pw, v.y, acc[r][j][1]);
+            acc[r][j][2] = fmaf(pw, v.z, acc[r][j][2]);
+            acc[r][j][3] = fmaf(pw, v.w, acc[r][j][3]);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RPT; ++r) {
+    const int row = u.row0 + rg * RPT + r;
+    if (row >= u.nrows) continue;
+    const int b = u.lo + row / p.R, h = u.hk * p.R + row % p.R;
+    const long long o = ((long long)u.slot * p.B + b) * p.Hq + h;
+    // An empty sequence has no part in its group's prefix.
+    const bool none = l[r] == 0.f || (u.group && p.seq_lens[b] <= 0);
+    const float inv = none ? 0.f : 1.f / l[r];
+    if (!none) {                                 // an empty part's O is not read
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (64 * j + 4 * c + e < d) p.part_o[o * d + 64 * j + 4 * c + e] = acc[r][j][e] * inv;
+    }
+    if (c == 0) p.part_lse[o] = none ? kNegInf : m[r] + log2f(l[r]);
+  }
+}
+
+// Partials: part_o [split_g + split_o][B * Hq][d], part_lse [split_g + split_o][B * Hq];
+// slots below split_g are the shared part's, the others the own part's.
+// Grid: x = unit of a KV head and split, y = KV head.  Units: the tiles of the groups' rows
+// (16 * rpt rows; sized for max_group), then the 16-row tiles of every sequence.
+template <typename T, int NJ>
 __global__ void __launch_bounds__(kThreads) units_kernel(const Params p, int group_tiles,
-                                                         int seq_tiles) {
-  extern __shared__ float sm[];
+                                                         int seq_tiles, int rpt) {
+  extern __shared__ __align__(16) float sm[];
   __shared__ int scratch[2];
-  const int d = p.d;
-  float* Qs = sm;                              // [16][d]
-  float* Ks = Qs + kRows * d;                  // [32][d + 1]
-  float* Vs = Ks + kTok * (d + 1);             // [32][d]
-  float* Ps = Vs + kTok * d;                   // [16][33]
-  const int split = blockIdx.x, hk = blockIdx.z;
-  const bool is_group = (int)blockIdx.y < p.G * group_tiles;
-  const int tid = threadIdx.x;
+  const int of_groups = p.G * group_tiles * p.split_g;
+  Unit u;
+  u.hk = blockIdx.y;
+  u.group = (int)blockIdx.x < of_groups;
+  const int splits = u.group ? p.split_g : p.split_o;
+  const int unit = ((int)blockIdx.x - (u.group ? 0 : of_groups)) / splits;
+  const int split = ((int)blockIdx.x - (u.group ? 0 : of_groups)) % splits;
   pdl_launch_dependents();
   pdl_wait();
 
-  int lo, nrows, row0, t_begin, t_end, table_row;
-  if (is_group) {
-    const int g = blockIdx.y / group_tiles, tile = blockIdx.y % group_tiles;
+  int t_begin, t_end;
+  if (u.group) {
+    const int g = unit / group_tiles, tile = unit % group_tiles;
     int hi, s, leader;
-    group_range(p, g, lo, hi);
-    row0 = tile * kRows;
-    nrows = (hi - lo) * p.R;
-    if (row0 >= nrows) return;
-    group_prefix(p, g, lo, hi, scratch, s, leader);
+    group_range(p, g, u.lo, hi);
+    u.row0 = tile * 16 * rpt;
+    u.nrows = (hi - u.lo) * p.R;
+    if (u.row0 >= u.nrows) return;
+    group_prefix(p, g, u.lo, hi, scratch, s, leader);
     if (s == 0) return;            // the sequences' own units mark the shared slots empty
     t_begin = 0;
     t_end = s;
-    table_row = leader;
+    u.table_row = leader;
   } else {
-    const int u = blockIdx.y - p.G * group_tiles;
-    lo = u / seq_tiles;
-    row0 = (u % seq_tiles) * kRows;
-    nrows = p.R;
-    const int g = group_of(p, lo, scratch);
+    u.lo = unit / seq_tiles;
+    u.row0 = (unit % seq_tiles) * 16;
+    u.nrows = p.R;
+    const int g = group_of(p, u.lo, scratch);
     int s = 0;
     if (g >= 0) {
       int glo, ghi, leader;
       group_range(p, g, glo, ghi);
       group_prefix(p, g, glo, ghi, scratch, s, leader);
     }
-    t_end = seq_len(p, lo, split == 0 && tid == 0);
+    t_end = seq_len(p, u.lo, split == 0 && threadIdx.x == 0);
     t_begin = min(s, t_end);
-    table_row = lo;
-    if (t_begin == 0 && tid < kRows && row0 + tid < nrows)   // no shared part
-      p.part_lse[((long long)split * p.B + lo) * p.Hq + hk * p.R + row0 + tid] =
-          __int_as_float(0xff800000);
+    u.table_row = u.lo;
+    if (t_begin == 0 && split == 0)   // no shared part
+      for (int i = threadIdx.x; i < 16 * p.split_g; i += kThreads)
+        if (u.row0 + (i & 15) < u.nrows)
+          p.part_lse[((long long)(i >> 4) * p.B + u.lo) * p.Hq + u.hk * p.R + u.row0 + (i & 15)] =
+              __int_as_float(0xff800000);
   }
   // this block's share of the tokens, in whole steps
   const int steps = (t_end - t_begin + kTok - 1) / kTok;
-  const int s0 = (int)((long long)steps * split / p.nsplit);
-  const int s1 = (int)((long long)steps * (split + 1) / p.nsplit);
-  const int first = t_begin + s0 * kTok, last = min(t_end, t_begin + s1 * kTok);
-
-  const int r = tid >> 4, c = tid & 15;
-  const int row = row0 + r;                       // row of the unit's row set
-  const int b = lo + row / p.R, h = hk * p.R + row % p.R;
-  const bool valid = row < nrows;
-  const T* q = reinterpret_cast<const T*>(p.q);
-  for (int i = c; i < d; i += 16)
-    Qs[r * d + i] = valid ? to_f32(q[((long long)b * p.Hq + h) * d + i]) * p.scale_log2 : 0.f;
-
-  const T* kp = reinterpret_cast<const T*>(p.k_pages);
-  const T* vp = reinterpret_cast<const T*>(p.v_pages);
-  const float kNegInf = __int_as_float(0xff800000);
-  float m = kNegInf, l = 0.f, acc[16];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) acc[j] = 0.f;
-
-  for (int t0 = first; t0 < last; t0 += kTok) {
-    const int nt = min(kTok, last - t0);
-    __syncthreads();
-    // 8 threads per token load its key and value
-    {
-      const int t = tid >> 3;
-      if (t < nt) {
-        const int tok = t0 + t;
-        const long long base =
-            (((long long)page_of(p, table_row, tok) * p.Hkv + hk) * p.P + tok % p.P) * d;
-        for (int i = tid & 7; i < d; i += 8) {
-          Ks[t * (d + 1) + i] = to_f32(kp[base + i]);
-          Vs[t * d + i] = to_f32(vp[base + i]);
-        }
-      } else {
-        for (int i = tid & 7; i < d; i += 8) {
-          Ks[t * (d + 1) + i] = 0.f;
-          Vs[t * d + i] = 0.f;
-        }
-      }
-    }
-    __syncthreads();
-    float x0 = 0.f, x1 = 0.f;
-    for (int i = 0; i < d; ++i) {
-      const float qv = Qs[r * d + i];
-      x0 = fmaf(qv, Ks[c * (d + 1) + i], x0);
-      x1 = fmaf(qv, Ks[(c + 16) * (d + 1) + i], x1);
-    }
-    if (c >= nt) x0 = kNegInf;
-    if (c + 16 >= nt) x1 = kNegInf;
-    float tm = fmaxf(x0, x1);
-#pragma unroll
-    for (int o = 8; o; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, o));
-    const float mn = fmaxf(m, tm);
-    const float mu = mn == kNegInf ? 0.f : mn;    // every score -inf: weights 0
-    const float f = exp2f(m - mu);
-    const float p0 = exp2f(x0 - mu), p1 = exp2f(x1 - mu);
-    float ps = p0 + p1;
-#pragma unroll
-    for (int o = 8; o; o >>= 1) ps += __shfl_xor_sync(0xffffffffu, ps, o);
-    l = l * f + ps;
-    m = mn;
-    Ps[r * (kTok + 1) + c] = p0;
-    Ps[r * (kTok + 1) + c + 16] = p1;
-    __syncwarp();                                 // a row's threads are in one warp
-#pragma unroll
-    for (int j = 0; j < 16; ++j) acc[j] *= f;
-    for (int t = 0; t < nt; ++t) {
-      const float w = Ps[r * (kTok + 1) + t];
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (c + 16 * j < d) acc[j] = fmaf(w, Vs[t * d + c + 16 * j], acc[j]);
-    }
-  }
-  if (!valid) return;
-  const int slot = (is_group ? 0 : p.nsplit) + split;
-  const long long o = ((long long)slot * p.B + b) * p.Hq + h;
-  // An empty sequence has no part in its group's prefix.
-  const bool none = l == 0.f || (is_group && p.seq_lens[b] <= 0);
-  const float inv = none ? 0.f : 1.f / l;
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (c + 16 * j < d) p.part_o[o * d + c + 16 * j] = none ? 0.f : acc[j] * inv;
-  if (c == 0) p.part_lse[o] = none ? kNegInf : m + log2f(l);
+  const int s0 = (int)((long long)steps * split / splits);
+  const int s1 = (int)((long long)steps * (split + 1) / splits);
+  u.first = t_begin + s0 * kTok;
+  u.last = min(t_end, t_begin + s1 * kTok);
+  u.slot = (u.group ? 0 : p.split_g) + split;
+  if (u.group && rpt == 4)
+    attend<T, NJ, 4>(p, u, sm);
+  else
+    attend<T, NJ, 1>(p, u, sm);
 }
 
 // One warp per row (b, h).
@@ -181,7 +269,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p) {
   const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= rows) return;
-  const int n = 2 * p.nsplit;
+  const int n = p.split_g + p.split_o;
   float M = __int_as_float(0xff800000);
   for (int i = 0; i < n; ++i) M = fmaxf(M, p.part_lse[i * rows + row]);
   float acc[8], L = 0.f;
@@ -221,18 +309,34 @@ Device device() {
   return d;
 }
 
-int generic_splits(int B, int Hq, int Hkv, int G, int max_group) {
-  // Splits of a unit's tokens: enough blocks for four per SM, at most 16.
-  const int R = Hq / Hkv;
-  const long long units = (long long)Hkv * ((long long)G * (((long long)max_group * R + 15) / 16) +
-                                            (long long)B * ((R + 15) / 16));
-  long long s = (4 * 148 + units - 1) / units;
+// Rows per thread of a group's units: 4 (64-row tiles) from 48 rows on, where a smaller tile
+// would read K and V more often than a larger one wastes rows.
+int generic_rpt(int Hq, int Hkv, int max_group) {
+  return (long long)max_group * (Hq / Hkv) >= 48 ? 4 : 1;
+}
+
+// Splits of `units` units' tokens: enough blocks for four per SM, at most 16.
+int generic_splits(long long units) {
+  const long long s = (4 * 148 + units - 1) / (units > 0 ? units : 1);
   return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
+}
+struct GenericPlan {
+  int rpt, group_tiles, seq_tiles, split_g, split_o;
+};
+GenericPlan generic_plan(int B, int Hq, int Hkv, int G, int max_group) {
+  GenericPlan z;
+  const int R = Hq / Hkv;
+  z.rpt = generic_rpt(Hq, Hkv, max_group);
+  z.group_tiles = (int)(((long long)max_group * R + 16 * z.rpt - 1) / (16 * z.rpt));
+  z.seq_tiles = (R + 15) / 16;
+  z.split_g = G ? generic_splits((long long)Hkv * G * z.group_tiles) : 1;
+  z.split_o = generic_splits((long long)Hkv * B * z.seq_tiles);
+  return z;
 }
 
 size_t generic_workspace(int B, int Hq, int Hkv, int d, int G, int max_group) {
-  const int s = generic_splits(B, Hq, Hkv, G, max_group);
-  return (size_t)2 * s * B * Hq * ((size_t)d + 1) * sizeof(float);
+  const GenericPlan z = generic_plan(B, Hq, Hkv, G, max_group);
+  return (size_t)(z.split_g + z.split_o) * B * Hq * ((size_t)d + 1) * sizeof(float);
 }
 
 // Workspace of the tensor-core kernels: plan, tables (if they do not fit shared memory),
@@ -305,27 +409,37 @@ static cudaError_t launch_chained(dim3 grid, dim3 block, size_t smem, cudaStream
   return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-template <typename T>
-static cudaError_t launch_generic(prefix::Params p, float* ws, std::string* err,
-                                  cudaStream_t stream) {
+template <typename T, int NJ>
+static cudaError_t launch_generic_d(prefix::Params p, float* ws, std::string* err,
+                                    cudaStream_t stream) {
   namespace gen = prefix::generic;
-  const int group_tiles = (int)(((long long)p.max_group * p.R + gen::kRows - 1) / gen::kRows);
-  const int seq_tiles = (p.R + gen::kRows - 1) / gen::kRows;
-  p.nsplit = generic_splits(p.B, p.Hq, p.Hkv, p.G, p.max_group);
+  const GenericPlan z = generic_plan(p.B, p.Hq, p.Hkv, p.G, p.max_group);
+  p.split_g = z.split_g;
+  p.split_o = z.split_o;
   p.part_o = ws;
-  p.part_lse = ws + (size_t)2 * p.nsplit * p.B * p.Hq * p.d;
-  const long long units = (long long)p.G * group_tiles + (long long)p.B * seq_tiles;
-  if (units > 65535 || p.Hkv > 65535) {
-    *err = "more than 65535 row tiles (groups x max_group, sequences) for this shape";
+  p.part_lse = ws + (size_t)(z.split_g + z.split_o) * p.B * p.Hq * p.d;
+  const long long blocks = (long long)p.G * z.group_tiles * z.split_g +
+                           (long long)p.B * z.seq_tiles * z.split_o;
+  if (blocks > INT_MAX || p.Hkv > 65535) {
+    *err = "too many row tiles (groups x max_group, sequences) for this shape";
     return cudaErrorInvalidConfiguration;
   }
-  cudaError_t e = launch_chained<gen::units_kernel<T>>(
-      dim3(p.nsplit, (unsigned)units, p.Hkv), dim3(gen::kThreads), gen::smem_bytes(p.d), stream, p,
-      group_tiles, seq_tiles);
+  cudaError_t e = launch_chained<gen::units_kernel<T, NJ>>(
+      dim3((unsigned)blocks, p.Hkv), dim3(gen::kThreads),
+      gen::smem_floats(z.rpt, 64 * NJ) * sizeof(float), stream, p, z.group_tiles, z.seq_tiles,
+      z.rpt);
   if (e != cudaSuccess) return e;
   const long long rows = (long long)p.B * p.Hq;
   return launch_chained<gen::join_kernel<T>>(dim3((unsigned)((rows + 7) / 8)), dim3(256), 0,
                                              stream, p);
+}
+
+template <typename T>
+static cudaError_t launch_generic(const prefix::Params& p, float* ws, std::string* err,
+                                  cudaStream_t stream) {
+  if (p.d <= 64) return launch_generic_d<T, 1>(p, ws, err, stream);
+  if (p.d <= 128) return launch_generic_d<T, 2>(p, ws, err, stream);
+  return launch_generic_d<T, 4>(p, ws, err, stream);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -454,7 +568,7 @@ cudaError_t launch_shared_prefix_decode(const void* q, const void* kp, const voi
   p.starts = starts; p.shared = shared; p.out = out; p.status = status;
   p.part_o = nullptr; p.part_lse = nullptr;
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.R = Hq / Hkv; p.d = d; p.P = P; p.max_pages = max_pages;
-  p.num_pages = num_pages; p.G = G; p.max_group = max_group; p.nsplit = 1;
+  p.num_pages = num_pages; p.G = G; p.max_group = max_group; p.split_g = p.split_o = 1;
   p.scale_log2 = scale * 1.4426950408889634f;
   auto al = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15) == 0; };
   if (!(flags & LLMC_DECODE_FORCE_GENERIC) && tc_shape(dtype, d, P, max_pages, B, Hq, Hkv, G) &&

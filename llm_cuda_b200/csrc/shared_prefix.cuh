@@ -29,7 +29,7 @@ struct Params {
   float* part_lse;
   int32_t* status;
   int B, Hq, Hkv, R, d, P, max_pages, num_pages, G, max_group;   // R = Hq / Hkv
-  int nsplit;
+  int split_g, split_o;        // splits of a group's shared tokens, of a sequence's own
   float scale_log2;            // softmax scale * log2(e)
 };
 
