@@ -65,14 +65,20 @@ struct TcParams {
 // units and ranges both ascend.  A slot is [D / 4][rows][4] fp32, so that the lanes of a
 // warp (rows) store 16-byte pieces side by side.
 
+// This kernel's code is fetched anew in every decode step (the weights that stream between two
+// launches push it out of the caches), some 200 cycles for every eight instructions.  So what
+// is not in an inner loop is kept small: loops are not unrolled, helpers are not inlined.
+
 // x / n for x >= 0, n > 0: the estimate is off by a few at most (24-bit mantissas).
-__device__ __forceinline__ int quot(int x, int n) {
+__device__ __noinline__ int quot(int x, int n) {
   int q = (int)(__int2float_rz(x) * __frcp_rn((float)n));
   int r = x - q * n;
+#pragma unroll 1
   while (r < 0) {
     --q;
     r += n;
   }
+#pragma unroll 1
   while (r >= n) {
     ++q;
     r -= n;
@@ -80,17 +86,33 @@ __device__ __forceinline__ int quot(int x, int n) {
   return q;
 }
 
-// What the chunks cost, in units of some 1100 cycles: a chunk of 128 rows at most 3 (K and V
-// of 64 KB at a fair share of the bandwidth are 2700 cycles), a chunk of a wide tile 4, and a
-// unit of own tokens 2 more, for the turn-over of a stream (measured: own units of n chunks
-// 2500 + 3400 n cycles, wide chunks 4400).  With few chunks for the CTAs every chunk is 1.
+// Waits for the barrier's phase of this parity.  Gives up after kWaits attempts (each lets the
+// warp sleep for up to microseconds), or when another warp has: the flag and the status word
+// say so, and every later wait returns at once.
+constexpr int kWaits = 1 << 20;
+__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                     int* status) {
+#pragma unroll 1
+  for (int i = 0; !mbar_try_wait(bar, parity); ++i) {
+    if (*abort_flag) break;
+    if (i == kWaits) {
+      *abort_flag = 1;
+      atomicOr(status, kStatusWaitTimeout);
+    }
+  }
+}
+
+// What the chunks cost, in units of some 450 cycles: a chunk of 128 rows at most 6 (K and V
+// of 64 KB at a fair share of the bandwidth are 2700 cycles), a chunk of a wide tile 11, and a
+// unit of own tokens 4 more, for the turn-over of a stream (fitted to the CTAs' end times).
+// With few chunks for the CTAs every chunk is 1.
 struct Costs {
   int shared, own, unit;
   __device__ __forceinline__ void set(int chunks, bool wide, int ctas) {
-    const bool few = chunks < 2 * ctas;   // otherwise every CTA's share exceeds own + unit
-    shared = few ? 1 : wide ? 4 : 3;
-    own = few ? 1 : 3;
-    unit = few ? 0 : 2;
+    const bool few = chunks < 2 * ctas;   // otherwise a CTA's share exceeds any chunk's cost
+    shared = few ? 1 : wide ? 11 : 6;
+    own = few ? 1 : 6;
+    unit = few ? 0 : 4;
   }
   // where chunk j of an own unit begins, and the first chunk that begins at x or later
   __device__ __forceinline__ int at(int j) const { return j ? unit + j * own : 0; }
@@ -113,10 +135,12 @@ struct Split {
   __device__ __forceinline__ int start(int c) const {   // floor(c total / C), c <= C
     return c * q + quot(c * r, C);
   }
-  __device__ __forceinline__ int owner(int x) const {   // the last c with start(c) <= x
+  __device__ __noinline__ int owner(int x) const {   // the last c with start(c) <= x
     const long long ec = (long long)(x + 1) * C;        // start(c) <= x  <=>  c total < (x + 1) C
     int c = min(C - 1, (int)((float)x * (float)C * __frcp_rn((float)total)));
+#pragma unroll 1
     while (c + 1 < C && (long long)(c + 1) * total < ec) ++c;
+#pragma unroll 1
     while (c > 0 && (long long)c * total >= ec) --c;
     return c;
   }
@@ -136,26 +160,37 @@ __device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr, int box) {
   return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) |
          ((uint64_t)(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t acc) {
+// The issuer's warp runs its loop as one and one elected lane (`el`) issues.  (With the loop in a
+// branch of one lane each product took some 20 cycles longer to issue.)
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t acc, uint32_t el) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(el)
       : "memory");
 }
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
-                                       uint32_t acc) {
+                                       uint32_t acc, uint32_t el) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
+      "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(el)
       : "memory");
 }
-__device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   bar)
-               : "memory");
+__device__ __forceinline__ void commit(uint32_t bar, uint32_t el) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(el)
+      : "memory");
 }
 __device__ __forceinline__ void fence_before() {
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -165,6 +200,23 @@ __device__ __forceinline__ void fence_after() {
 }
 __device__ __forceinline__ void wait_ld() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// Loads are asynchronous: the registers hold the values behind wait_ld(), and the compiler may
+// use them only behind this, which ties their uses to the wait.
+__device__ __forceinline__ void landed(uint32_t (&r)[32]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]),
+                 "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ void landed(uint32_t (&r)[16]) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]),
+                 "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                 "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
 }
 __device__ __forceinline__ void wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -191,19 +243,6 @@ __device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
         "=r"(r[14]), "=r"(r[15])
       : "r"(addr)
-      : "memory");
-}
-__device__ __forceinline__ void st32(uint32_t addr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(
-          addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-      "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
 __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
@@ -241,6 +280,16 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+__device__ __forceinline__ float block_max(const uint32_t (&v)[2][32]) {
+  float a = __uint_as_float(v[0][0]), b = __uint_as_float(v[1][0]);
+#pragma unroll
+  for (int e = 1; e < 31; e += 2) {
+    a = fmaxf(a, fmaxf(__uint_as_float(v[0][e]), __uint_as_float(v[0][e + 1])));
+    b = fmaxf(b, fmaxf(__uint_as_float(v[1][e]), __uint_as_float(v[1][e + 1])));
+  }
+  return fmaxf(fmaxf(a, b), fmaxf(__uint_as_float(v[0][31]), __uint_as_float(v[1][31])));
 }
 
 template <int D>
@@ -294,6 +343,7 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
   const Params& p = tp.p;
   const int lane = tid & 31;
   // The last warps fetch the groups, the others the lengths: one round trip for both.
+#pragma unroll 1
   for (int g = nt - 1 - tid; g <= p.G; g += nt) {
     t.lo[g] = p.G ? p.starts[g] : 0;
     if (g < p.G) {
@@ -302,13 +352,16 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
       t.unit[g] = p.shared[g];
     }
   }
+#pragma unroll 1
   for (int b = tid; b < p.B; b += nt) t.len[b] = seq_len(p, b, true);
   bar1(nt);
+#pragma unroll 1
   for (int b = tid; b < p.B; b += nt) {
     const int n = t.len[b];
     int gid = -1;
     if (p.G) {
       int a = 0, z = p.G;     // the last group that starts at or before b
+#pragma unroll 1
       while (z - a > 1) {
         const int mid = (a + z) >> 1;
         if (t.lo[mid] <= b) a = mid; else z = mid;
@@ -326,6 +379,7 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
   if (tid < 32) {   // the groups, with prefix sums for narrow and for wide tiles
     // One bad range and nothing is shared: overlapping groups would pass the workspace.
     int bad = 0;
+#pragma unroll 1
     for (int g = lane; g < p.G; g += 32)
       bad |= t.lo[g] < 0 || t.lo[g + 1] < t.lo[g] || t.lo[g + 1] > p.B;
     bad = __any_sync(0xffffffffu, bad);
@@ -333,6 +387,7 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
     const int narrow = tp.nb * p.R;
     const int per = (p.G + 31) >> 5, g0 = min(lane * per, p.G), g1 = min(g0 + per, p.G);
     int w0 = 0, w1 = 0, u0 = 0, u1 = 0, most = 0;
+#pragma unroll 1
     for (int g = g0; g < g1; ++g) {   // a lane's groups with either tile
       int n = 0, rows = 0;
       if (!bad && t.leader[g] != 0x7fffffff) {
@@ -357,6 +412,7 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
     const int bper = (p.B + 31) >> 5, b0 = min(lane * bper, p.B), b1 = min(b0 + bper, p.B);
     __syncwarp();
     int oc = 0, ou = 0;
+#pragma unroll 1
     for (int b = b0; b < b1; ++b) {
       int gid = t.gid[b];
       if (gid >= 0 && t.s[gid] == 0) t.gid[b] = gid = -1;
@@ -370,7 +426,7 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
     const int wl = (wide ? w1 : w0) * cost.shared, ul = wide ? u1 : u0;
     const int xl = oc * cost.own + ou * cost.unit;
     int cs = wl, us = ul, xs = xl;
-#pragma unroll
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
       const int a = __shfl_up_sync(0xffffffffu, cs, o), b = __shfl_up_sync(0xffffffffu, us, o);
       const int d = __shfl_up_sync(0xffffffffu, xs, o);
@@ -389,6 +445,7 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
     cs -= wl;
     us -= ul;
     xs -= xl;
+#pragma unroll 1
     for (int g = g0; g < g1; ++g) {
       t.start[g] = cs;
       t.unit[g] = us;
@@ -398,6 +455,7 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
         cs += ta * ((t.s[g] + kChunk - 1) / kChunk) * cost.shared;
       }
     }
+#pragma unroll 1
     for (int b = b0; b < b1; ++b) {
       t.own[b] = xs;
       const int gid = t.gid[b], n = own_chunks(p, gid >= 0 ? t.s[gid] : 0, t.len[b]);
@@ -408,7 +466,7 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
 }
 
 // The plan's entries first, first + step, ...
-__device__ __forceinline__ void write_plan(const TcParams& tp, const Tables& t, const int* totals,
+__device__ __noinline__ void write_plan(const TcParams& tp, const Tables& t, const int* totals,
                                            int ctas, int first, int step) {
   const Params& p = tp.p;
   const int narrow = tp.nb * p.R, rt = totals[2];
@@ -416,6 +474,7 @@ __device__ __forceinline__ void write_plan(const TcParams& tp, const Tables& t, 
   split.set(totals[1], ctas);
   Costs cost;
   cost.set(totals[3], rt > narrow, ctas);
+#pragma unroll 1
   for (int e = first; e < p.B * p.Hkv; e += step) {
     const int b = quot(e, p.Hkv), hk = e - b * p.Hkv, g = t.gid[b];
     int4 v = make_int4(0, 0, 0, 0);
@@ -473,9 +532,10 @@ struct Walker {
   Costs cost;
 
   // The last of n ascending entries that is <= x (0 if none), by a whole warp.
-  static __device__ __forceinline__ int find(const int* a, int n, int x) {
+  static __device__ __noinline__ int find(const int* a, int n, int x) {
     const int lane = threadIdx.x & 31;
     int lo = 0;
+#pragma unroll 1
     while (n > 1) {
       const int step = (n + 31) >> 5, i = lane * step;
       const int k = __popc(__ballot_sync(0xffffffffu, i < n && a[lo + i] <= x));
@@ -500,10 +560,12 @@ struct Walker {
   }
   __device__ __forceinline__ bool next(const TcParams& tp, const Tables& t, Segment& sg) {
     const Params& p = tp.p;
+#pragma unroll 1
     while (x < x1) {
       int j0, j1;
       if (x < X0) {
         int nch, tiles, size;
+#pragma unroll 1
         while (true) {   // the group that holds x
           nch = (t.s[g] + kChunk - 1) / kChunk;
           tiles = quot(t.rows[g] + rt - 1, rt);
@@ -528,6 +590,7 @@ struct Walker {
         sg.slot = 2 * (t.unit[g] + ul + (int)blockIdx.x);
       } else {
         int nch, s, size;
+#pragma unroll 1
         while (true) {   // the sequence that holds x
           s = t.gid[b] >= 0 ? t.s[t.gid[b]] : 0;
           nch = own_chunks(p, s, t.len[b]);
@@ -655,20 +718,21 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     int k = 0, qc = 0;
     Walker w0;
     if (!isv) w0.init(tp, t, totals);
+#pragma unroll 1
     for (int ns = 0;; ++ns) {
       Segment sg;
       const int slot = ns % kRing;
       Segment* entry = reinterpret_cast<Segment*>(smem + S::kSegs) + slot;
       if (!isv) {
         if (!w0.next(tp, t, sg)) sg.n = 0;
-        mbar_wait_bounded(gempty + 8 * slot, ((ns / kRing) & 1) ^ 1, abort_flag, p.status);
+        wait(gempty + 8 * slot, ((ns / kRing) & 1) ^ 1, abort_flag, p.status);
         if (lane == 0) {
           *entry = sg;
           mbar_arrive(gfull + 8 * slot);
         }
         __syncwarp();
       } else {
-        mbar_wait_bounded(gfull + 8 * slot, (ns / kRing) & 1, abort_flag, p.status);
+        wait(gfull + 8 * slot, (ns / kRing) & 1, abort_flag, p.status);
         sg = *entry;
         __syncwarp();
         if (lane == 0) mbar_arrive(gempty + 8 * slot);
@@ -682,9 +746,10 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
       };
       int next = page_at(0);
       if (!isv) {
+#pragma unroll 1
         for (int q = 0; q <= sg.wide; ++q, ++qc) {
           const int qb = qc & 1;
-          mbar_wait_bounded(qempty + 8 * qb, ((qc >> 1) & 1) ^ 1, abort_flag, p.status);
+          wait(qempty + 8 * qb, ((qc >> 1) & 1) ^ 1, abort_flag, p.status);
           if (lane == 0 && !*abort_flag) {
             mbar_arrive_expect_tx(qfull + 8 * qb, (uint32_t)((sg.own ? 1 : tp.nb) * p.R * D * 2));
 #pragma unroll
@@ -695,6 +760,7 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
           __syncwarp();
         }
       }
+#pragma unroll 1
       for (int j = 0; j < sg.n; ++j, ++k) {
         const int st = k % NS;
         const int t0 = sg.t0 + j * kChunk;
@@ -708,7 +774,7 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         int in_page = 0;      // a page of more than a chunk: where in it
         if (p.P > kChunk) in_page = t0 - quot(t0, p.P) * p.P;
         const int y = (page * p.Hkv + sg.hk) * p.P + in_page;   // pool rows: below 2^31
-        mbar_wait_bounded(empties + 8 * st, ((k / NS) & 1) ^ 1, abort_flag, p.status);
+        wait(empties + 8 * st, ((k / NS) & 1) ^ 1, abort_flag, p.status);
         const bool go = !*abort_flag;
         const uint32_t full = fulls + 8 * st;
         if (lane == 0 && go) mbar_arrive_expect_tx(full, (uint32_t)(boxes * box * D * 2));
@@ -736,42 +802,68 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
   } else if (warp == 9) {
     // ---- tcgen05 issuer ----
     asm volatile("bar.sync 2, 288;" ::: "memory");   // the softmax warps' rehearsal is over
-    if (lane == 0) {
-      // Segment entries are read once by each cursor; b's read gives the entry back.
-      auto load = [&](Cursor& c, bool last) {
-        const int slot = c.seg % kRing;
-        mbar_wait_bounded(gfull + 8 * slot, (c.seg / kRing) & 1, abort_flag, p.status);
-        const int4 v = *reinterpret_cast<const int4*>(smem + S::kSegs + 48 * slot);
-        c.n = *abort_flag ? 0 : v.x;
-        c.wide = v.y; c.t0 = v.z; c.hi = v.w;
-        c.j = 0;
-        if (last) mbar_arrive(gempty + 8 * slot);
-        ++c.seg;
-      };
-      auto advance = [&](Cursor& c, bool last) {
-        ++c.item;
-        if (c.wide && c.sub == 0) {
-          c.sub = 1;
-          return;
+    const uint32_t el = elect_one();
+    // Segment entries are read once by each cursor; b's read gives the entry back.
+    auto load = [&](Cursor& c, bool last) {
+      const int slot = c.seg % kRing;
+      wait(gfull + 8 * slot, (c.seg / kRing) & 1, abort_flag, p.status);
+      const int4 v = *reinterpret_cast<const int4*>(smem + S::kSegs + 48 * slot);
+      c.n = *abort_flag ? 0 : v.x;
+      c.wide = v.y; c.t0 = v.z; c.hi = v.w;
+      c.j = 0;
+      __syncwarp();
+      if (last && el) mbar_arrive(gempty + 8 * slot);
+      ++c.seg;
+    };
+    auto advance = [&](Cursor& c, bool last) {
+      ++c.item;
+      if (c.wide && c.sub == 0) {
+        c.sub = 1;
+        return;
+      }
+      c.sub = 0;
+      ++c.k;
+      if (++c.j == c.n) {
+        c.qc += 1 + c.wide;
+        load(c, last);
+      }
+    };
+    // 32-token blocks of the current chunk that hold tokens
+    auto blocks = [](const Cursor& c) { return (min(kChunk, c.hi - c.t0 - c.j * kChunk) + 31) >> 5; };
+    // V: 16 tokens of a k-step are inside a box, or two boxes of 8 (descriptor units of 16 B)
+    const int vbox = min(p.P, kChunk), vsh = 31 - __clz(vbox), vstep = vbox * 8 * S::kHalves;
+    Cursor a = {}, b = {};     // S (a) runs two items ahead of P V (b)
+    load(a, false);
+    load(b, true);
+    uint32_t ready = 0;        // bit s: parity of stream s's next P
+#pragma unroll 1
+    for (int lead = 2; b.n;) {
+      if (lead) {
+        --lead;
+      } else {                 // O += P V
+        const int s = b.item & 1, st = b.k % NS;
+        wait(pready + 8 * s, (ready >> s) & 1, abort_flag, p.status);
+        if (b.sub == 0) wait(vfull + 8 * st, (b.k / NS) & 1, abort_flag, p.status);
+        fence_after();
+        const uint64_t vd = desc_mnmajor(sb + S::kV + st * S::kOperand, vbox);
+        const bool first = b.wide ? b.j == 0 : b.j < 2;
+        const int steps = 2 * blocks(b);
+#pragma unroll
+        for (int kk = 0; kk < kChunk / 16; ++kk) {
+          if (kk >= steps) continue;
+          mma_ts(tmem + 256 + s * D, tmem + s * 128 + kk * 8,
+                 vd + (((kk * 16) >> vsh) * vstep + ((kk * 16) & (vbox - 1)) * 8), ID_O,
+                 !first || kk > 0, el);
         }
-        c.sub = 0;
-        ++c.k;
-        if (++c.j == c.n) {
-          c.qc += 1 + c.wide;
-          load(c, last);
-        }
-      };
-      // 32-token blocks of the current chunk that hold tokens
-      auto blocks = [](const Cursor& c) { return (min(kChunk, c.hi - c.t0 - c.j * kChunk) + 31) >> 5; };
-      // V: 16 tokens of a k-step are inside a box, or two boxes of 8 (descriptor units of 16 B)
-      const int vbox = min(p.P, kChunk), vsh = 31 - __clz(vbox), vstep = vbox * 8 * S::kHalves;
-      Cursor a = {}, b = {};     // S (a) runs two items ahead of P V (b)
-      load(a, false);
-      uint32_t ready = 0;        // bit s: parity of stream s's next P
-      auto issue_s = [&]() {
+        ready ^= 1u << s;
+        if (!b.wide || b.sub == 1) commit(vempty + 8 * st, el);
+        if (b.wide ? b.j == b.n - 1 : b.j >= b.n - 2) commit(ofull + 8 * s, el);
+        advance(b, true);
+      }
+      if (a.n) {               // S = Q K^T
         const int s = a.item & 1, st = a.k % NS, qi = a.qc + a.sub, qb = qi & 1;
-        if (a.j == 0) mbar_wait_bounded(qfull + 8 * qb, (qi >> 1) & 1, abort_flag, p.status);
-        if (a.sub == 0) mbar_wait_bounded(kfull + 8 * st, (a.k / NS) & 1, abort_flag, p.status);
+        if (a.j == 0) wait(qfull + 8 * qb, (qi >> 1) & 1, abort_flag, p.status);
+        if (a.sub == 0) wait(kfull + 8 * st, (a.k / NS) & 1, abort_flag, p.status);
         fence_after();
         const uint64_t qd = desc_kmajor(sb + S::kQ + qb * S::kOperand);
         const uint64_t kd = desc_kmajor(sb + S::kK + st * S::kOperand);
@@ -779,35 +871,12 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = ((kk / 4) * S::kTile + (kk % 4) * 32) >> 4;
-          mma_ss(tmem + s * 128, qd + off, kd + off, id, kk > 0);
+          mma_ss(tmem + s * 128, qd + off, kd + off, id, kk > 0, el);
         }
-        commit(sfull + 8 * s);
-        if (!a.wide || a.sub == 1) commit(kempty + 8 * st);
-        if (a.j == a.n - 1) commit(qempty + 8 * qb);
+        commit(sfull + 8 * s, el);
+        if (!a.wide || a.sub == 1) commit(kempty + 8 * st, el);
+        if (a.j == a.n - 1) commit(qempty + 8 * qb, el);
         advance(a, false);
-      };
-      if (a.n) issue_s();
-      if (a.n) issue_s();
-      load(b, true);
-      while (b.n) {
-        const int s = b.item & 1, st = b.k % NS;
-        mbar_wait_bounded(pready + 8 * s, (ready >> s) & 1, abort_flag, p.status);
-        ready ^= 1u << s;
-        if (b.sub == 0) mbar_wait_bounded(vfull + 8 * st, (b.k / NS) & 1, abort_flag, p.status);
-        fence_after();
-        const uint64_t vd = desc_mnmajor(sb + S::kV + st * S::kOperand, vbox);
-        const bool first = b.wide ? b.j == 0 : b.j < 2;
-        const int nb = blocks(b);
-#pragma unroll
-        for (int kk = 0; kk < kChunk / 16; ++kk)
-          if (kk < 2 * nb)
-            mma_ts(tmem + 256 + s * D, tmem + s * 128 + kk * 8,
-                   vd + (((kk * 16) >> vsh) * vstep + ((kk * 16) & (vbox - 1)) * 8), ID_O,
-                   !first || kk > 0);
-        if (!b.wide || b.sub == 1) commit(vempty + 8 * st);
-        if (b.wide ? b.j == b.n - 1 : b.j >= b.n - 2) commit(ofull + 8 * s);
-        if (a.n) issue_s();
-        advance(b, true);
       }
     }
     __syncwarp();
@@ -836,7 +905,7 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
       const bool real = ns >= 0;
       if (real) {
         const int slot = ns % kRing;
-        mbar_wait_bounded(gfull + 8 * slot, (ns / kRing) & 1, abort_flag, p.status);
+        wait(gfull + 8 * slot, (ns / kRing) & 1, abort_flag, p.status);
         const int4* e = reinterpret_cast<const int4*>(segs + slot);
         const int4 x = e[0], y = e[1];
         sg.n = x.x; sg.wide = x.y; sg.t0 = x.z; sg.hi = x.w;
@@ -858,67 +927,66 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         const int t0 = sg.t0 + j * kChunk;
         const int hi = min(kChunk, sg.hi - t0), lo = max(0, sg.lo - t0);
         const int nb = (hi + 31) >> 5;
-        if (real) mbar_wait_bounded(sfull + 8 * s, n_items & 1, abort_flag, p.status);
+        if (real) wait(sfull + 8 * s, n_items & 1, abort_flag, p.status);
         fence_after();
         if (warp_on) {
-          // Two passes over S in TMEM, 64 columns at a time: little code, few registers.
-          float mx = kNegInf;
+          // Tokens outside the unit: -inf in TMEM, in the few blocks that have any.
+          if (lo > 0 || hi < kChunk) {
 #pragma unroll 1
-          for (int x = 0; x < kChunk; x += 64) {
-            if (x >= 32 * nb) break;
-            uint32_t v[2][32];
-            ld32(ts + x, v[0]);
-            ld32(ts + x + 32, v[1]);     // past nb: old columns, masked
-            wait_ld();
-            if (x < lo || x + 64 > hi) {   // tokens outside the unit: -inf, also for pass two
+            for (int x = 0; x < ((hi + 63) & ~63); x += 16) {
+              if (x >= lo && x + 16 <= hi) continue;
+              uint32_t o[16];
+              ld16(ts + x, o);
+              wait_ld();
+              landed(o);
 #pragma unroll
-              for (int e = 0; e < 64; ++e)
-                if (x + e < lo || x + e >= hi) v[e / 32][e % 32] = __float_as_uint(kNegInf);
-              st32(ts + x, v[0]);
-              st32(ts + x + 32, v[1]);
-              wait_st();
+              for (int e = 0; e < 16; ++e)
+                if (x + e < lo || x + e >= hi) o[e] = __float_as_uint(kNegInf);
+              st16(ts + x, o);
             }
-            float m0 = kNegInf, m1 = kNegInf;
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              m0 = fmaxf(m0, fmaxf(__uint_as_float(v[0][e]), __uint_as_float(v[0][e + 1])));
-              m1 = fmaxf(m1, fmaxf(__uint_as_float(v[1][e]), __uint_as_float(v[1][e + 1])));
-            }
-            mx = fmaxf(mx, fmaxf(m0, m1));
+            wait_st();
           }
-          // Raise the reference maximum when the weights would pass 2^8.
-          const bool start = j == first;
+          const bool start = j == first, two = nb > 2;
+          uint32_t v0[2][32], v1[2][32], w[2][16];
+          ld32(ts, v0[0]);
+          ld32(ts + 32, v0[1]);
+          if (two) {
+            ld32(ts + 64, v1[0]);
+            ld32(ts + 96, v1[1]);
+          }
+          wait_ld();
+          landed(v0[0]);
+          landed(v0[1]);
+          float mx = block_max(v0);
+          if (two) {
+            landed(v1[0]);
+            landed(v1[1]);
+            mx = fmaxf(mx, block_max(v1));
+          }
+          // Raise the reference maximum where the weights would pass 2^8.
           const bool raise = start || (mx - m) * sc > 8.f;
           if (__any_sync(0xffffffffu, raise)) {
-            float f = 1.f;
-            if (raise) {
-              f = start || m == kNegInf ? 0.f : ex2((m - mx) * sc);
-              m = mx;
-              float a, b;
-              unpair(l2, a, b);
-              l2 = pair(a * f, b * f);
-            }
+            const float f = !raise ? 1.f : m == kNegInf ? 0.f : ex2((m - mx) * sc);
+            m = raise ? mx : m;
+            float a, b;
+            unpair(l2, a, b);
+            l2 = pair(a * f, b * f);
             if (!start) {
 #pragma unroll 1
-              for (int x = 0; x < D / 16; ++x) {
+              for (int y = 0; y < D; y += 16) {
                 uint32_t o[16];
-                ld16(to + 16 * x, o);
+                ld16(to + y, o);
                 wait_ld();
+                landed(o);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                st16(to + 16 * x, o);
+                st16(to + y, o);
               }
             }
           }
           const float ms = m == kNegInf ? 0.f : m * sc;
           const uint64_t nm2 = pair(-ms, -ms);
-#pragma unroll 1
-          for (int x = 0; x < kChunk; x += 64) {
-            if (x >= 32 * nb) break;
-            uint32_t v[2][32], w[2][16];
-            ld32(ts + x, v[0]);
-            ld32(ts + x + 32, v[1]);
-            wait_ld();
+          auto weigh = [&](const uint32_t (&v)[2][32]) {
 #pragma unroll
             for (int e = 0; e < 64; e += 2) {
               float a, b;
@@ -929,9 +997,14 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
               l2 = add2(l2, pair(a, b));
               w[e / 32][e % 32 / 2] = Mma<T>::pack(a, b);
             }
-            // P's columns x / 2 .. x / 2 + 31 lie over S columns that have been read
-            st16(ts + x / 2, w[0]);
-            st16(ts + x / 2 + 16, w[1]);
+          };
+          weigh(v0);               // P's columns lie over S columns that have been read
+          st16(ts, w[0]);
+          st16(ts + 16, w[1]);
+          if (two) {
+            weigh(v1);
+            st16(ts + 32, w[0]);
+            st16(ts + 48, w[1]);
           }
           wait_st();
         }
@@ -941,7 +1014,7 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             // NaN.  S of this item follows the products of the stream's item before, so the
             // stage's earlier chunk is done: this wait cannot take its phase for the chunk's.
             const int st = (k + j) % NS;
-            mbar_wait_bounded(vfull + 8 * st, ((k + j) / NS) & 1, abort_flag, p.status);
+            wait(vfull + 8 * st, ((k + j) / NS) & 1, abort_flag, p.status);
             const uint32_t v0 = sb + S::kV + st * S::kOperand;
             const int per = (32 * nb - hi) * 8;
 #pragma unroll 1
@@ -968,7 +1041,7 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
       const bool write = real && r < rows;
       if (first < sg.n) {
         if (real) {
-          mbar_wait_bounded(ofull + 8 * s, n_o & 1, abort_flag, p.status);
+          wait(ofull + 8 * s, n_o & 1, abort_flag, p.status);
           ++n_o;
         }
         fence_after();
@@ -982,6 +1055,7 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             uint32_t o[32];
             ld32(to + 32 * x, o);
             wait_ld();
+            landed(o);
             if (write) {
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
