@@ -40,7 +40,7 @@ from ...kernels.decode_attention import (
     paged_decode_attention,
     rope_append_decode,
 )
-from ...kernels.beam import beam_reorder
+from ...kernels.beam import MAX_BEAMS, beam_reorder
 from ...kernels.rope import rope_append
 from ...kernels.shared_prefix import shared_prefix_decode
 from .rotary import RopeTable
@@ -344,6 +344,8 @@ class BeamKVCache(PagedKVCache):
                  generator: torch.Generator | None = None):
         if not prompt_lens:
             raise ValueError("prompt_lens must not be empty")
+        if not 1 <= beams <= MAX_BEAMS:
+            raise ValueError(f"a prompt has 1 to {MAX_BEAMS} beams")
         if max(prompt_lens) > max_seq_len or min(prompt_lens) < 1:
             raise ValueError("prompts must have 1 to max_seq_len tokens")
         device = torch.device(device)

@@ -133,3 +133,11 @@ def test_beam_cache_layout_and_refusals():
     with pytest.raises(ValueError, match="pools must be"):
         PagedKVLayerCache(2, 64, 64, 16, "cpu", torch.bfloat16, key_pages=kv[:3],
                           value_pages=kv[:3])
+
+
+@pytest.mark.parametrize("beams", [0, 33])
+def test_beam_cache_refuses_more_beams_than_the_kernels_take(beams):
+    from llm_cuda_b200.models.llama3 import BeamKVCache
+
+    with pytest.raises(ValueError, match="1 to 32 beams"):
+        BeamKVCache(1, 2, 64, 40, 16, "cpu", torch.bfloat16, [20], beams)
