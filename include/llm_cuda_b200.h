@@ -301,7 +301,7 @@ LLMC_API int llmc_shared_prefix_decode(
  *   A beam whose score, or whose log-sum-exp, is not finite (a NaN or +inf among its
  *     logits, all of them -inf) offers its tokens at -inf.
  *   out_scores [G, n] fp32, out_beams [G, n] int32 (0 .. K-1), out_tokens [G, n] int64.
- * 1 <= K <= 32, 1 <= n <= 64, n <= K * V.  Ranked in fp64, scores rounded once to fp32.
+ * 1 <= K <= 32, 1 <= V <= 2^27, 1 <= n <= 64, n <= K * V.  Ranked in fp64, scores rounded once to fp32.
  * One launch, no workspace.
  */
 LLMC_API int llmc_beam_select(const void* logits, long long row_stride, const float* beam_scores,

@@ -9,8 +9,8 @@
 // elements, more in long rows) in shared memory.  The order inside a row is that of its
 // logits, which needs no log-sum-exp, so the n best can be found before it is known: at
 // least n elements reach the n-th largest of the (pairs of) threads' maxima, and only the
-// few cells that reach it are read again.  Ranks come from comparing all pairs of the few survivors
-// (rows of very many equal logits go through sorted lists instead).  The cluster's first
+// few cells that reach it are read again.  Ranks come from comparing all pairs of the few
+// survivors (rows of very many equal logits go through sorted lists instead).  The cluster's first
 // CTA fetches the tasks' lists and sums through distributed shared memory and ranks the
 // candidates by their scores in the same way.
 // Bound: the logits are read once from HBM; then the exponentials (16 a cycle and SM).
@@ -32,7 +32,7 @@ namespace beam {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxBeams = 32;
+constexpr int kMaxBeams = 32;   // five bits of a candidate's tie
 constexpr int kU = 4;           // 16-byte vectors of a tile per lane; two more tiles in flight
 constexpr int kCells = 32;      // cells of a thread
 
@@ -62,9 +62,9 @@ __device__ __forceinline__ unsigned long long ld_dsmem_u64(uint32_t addr) {
 }
 
 // Order-preserving bits of a float, then the complemented index: larger is better, equal
-// values rank by the lowest index.  Never zero for a number (0 means "no entry").
+// values (0 and -0 too) rank by the lowest index.  Never zero for a number (0: "no entry").
 __device__ __forceinline__ unsigned long long make_key(float f, uint32_t idx) {
-  uint32_t u = __float_as_uint(f);
+  uint32_t u = __float_as_uint(f + 0.f);
   u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
   return ((unsigned long long)u << 32) | (0xFFFFFFFFu - idx);
 }
@@ -253,11 +253,17 @@ __device__ __noinline__ void merge_warps(const unsigned long long* buf, const in
   }
 }
 
-// A candidate: its fp64 score as bits that order like it, and beam << 32 | token, of which
-// the lower is better.
+// A candidate: its fp64 score as bits that order like it (0: no entry), and what decides
+// between equal ones, the lower the better: beam, falling logit, token.  (Logits of a beam
+// may differ by less than its scores can show; their order is that of the logits' lists,
+// which is what merging these relies on.)
+constexpr int kTokenBits = 27;
 struct __align__(16) Cand {
   unsigned long long score, tie;
 };
+__device__ __forceinline__ unsigned long long make_tie(int beam, uint32_t logit, uint32_t token) {
+  return (unsigned long long)beam << 59 | (unsigned long long)~logit << kTokenBits | token;
+}
 __device__ __forceinline__ unsigned long long score_bits(double x) {
   const unsigned long long u = (unsigned long long)__double_as_longlong(x + 0.0);   // no -0
   return u >> 63 ? ~u : u | 1ull << 63;
@@ -586,13 +592,15 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
     const int t = i / n, j = i - t * n, k = t / S;
     Cand c;
     double sc = -INFINITY;
-    c.tie = (1ull << 62) + i;            // no entry
+    c.score = 0ull;                      // no entry
+    c.tie = i;
     const int kind = row_kind[k];
     if (kind == 0) {
       const unsigned long long key = all[i];
       if (key != 0ull) {
         sc = row_b[k] + ((double)key_value(key) - row_lse[k]);
-        c.tie = (unsigned long long)k << 32 | key_index(key);
+        c.score = score_bits(sc);
+        c.tie = make_tie(k, (uint32_t)(key >> 32), key_index(key));
       }
     } else if (t == k * S) {
       int tok = j;
@@ -600,9 +608,11 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
         tok = j == 0 ? p.eos : j - 1 < p.eos ? j - 1 : j;
         if (j == 0) sc = row_b[k];
       }
-      if (tok < V) c.tie = (unsigned long long)k << 32 | (uint32_t)tok;
+      if (tok < V) {
+        c.score = score_bits(sc);
+        c.tie = make_tie(k, 0u, (uint32_t)tok);
+      }
     }
-    c.score = score_bits(sc);
     cand[i] = c;
   }
   __syncthreads();
@@ -663,8 +673,8 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
     const long long o = (long long)g * n + r;
     const Cand c = src[r];
     p.out_scores[o] = (float)bits_score(c.score);
-    p.out_beams[o] = (int32_t)(c.tie >> 32);
-    p.out_tokens[o] = (int64_t)(uint32_t)c.tie;
+    p.out_beams[o] = (int32_t)(c.tie >> 59);
+    p.out_tokens[o] = (int64_t)(c.tie & ((1ull << kTokenBits) - 1));
   }
 }
 

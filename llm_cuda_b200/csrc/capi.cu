@@ -453,7 +453,7 @@ int llmc_beam_select(const void* logits, long long row_stride, const float* beam
   if (!valid_dtype(dtype)) return fail(LLMC_EINVAL, "llmc_beam_select: unknown dtype");
   if (G < 0 || G > (1 << 24) || K < 1 || K > 32 || V < 1)
     return fail(LLMC_EINVAL, "llmc_beam_select: need 0 <= G <= 2^24, 1 <= K <= 32, V >= 1");
-  if (V > INT_MAX - 64) return fail(LLMC_EUNSUPPORTED, "llmc_beam_select: V too large");
+  if (V > 1 << 27) return fail(LLMC_EUNSUPPORTED, "llmc_beam_select: V > 2^27");
   if (n < 1 || n > 64 || (long long)n > (long long)K * V)
     return fail(LLMC_EINVAL, "llmc_beam_select: need 1 <= n <= 64 and n <= K * V");
   if (row_stride < V) return fail(LLMC_EINVAL, "llmc_beam_select: row_stride smaller than V");

@@ -73,6 +73,25 @@ def test_select_ties_go_to_the_lowest_beam_and_token():
     check_select(x, s, 33)
 
 
+def test_select_zeros_of_both_signs_are_equal():
+    x = torch.zeros(3, 1500, device=DEV)
+    x[:, ::2] = -0.0
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        check_select(x.to(dtype), torch.tensor([[-2.0, -1.0, -2.0]], device=DEV), 20)
+
+
+@pytest.mark.parametrize("n", [8, 64])
+def test_select_logits_closer_than_scores(n):
+    """Logits of 1e-22 and less: all scores round to -log(V), the order stays the logits'."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    row = torch.randperm(5000, generator=g, device=DEV).float() * 1e-26
+    x = row.repeat(8, 1)
+    s, b, t = beam_select(x, torch.zeros(1, 8, device=DEV), num_out=n)
+    assert (b == 0).all()
+    assert torch.equal(t[0], torch.argsort(row, descending=True)[:n])
+    assert ((s + math.log(5000)).abs() <= 2.0 ** -19).all()   # 2^-20 and fp32 of 8.5
+
+
 def test_select_sorted_rows():
     """Ascending logits make every tile better than all before it; descending ones none."""
     base = torch.arange(30000, device=DEV, dtype=torch.float32) / 1000

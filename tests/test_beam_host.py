@@ -141,3 +141,9 @@ def test_beam_cache_refuses_more_beams_than_the_kernels_take(beams):
 
     with pytest.raises(ValueError, match="1 to 32 beams"):
         BeamKVCache(1, 2, 64, 40, 16, "cpu", torch.bfloat16, [20], beams)
+
+
+def test_beam_select_refuses_a_vocabulary_past_its_ties():
+    lib = N.load()
+    assert _select(lib, V=(1 << 27) + 1, stride=1 << 28) == -2
+    assert b"2^27" in lib.llmc_last_error_string()
