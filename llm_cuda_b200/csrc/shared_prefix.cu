@@ -372,7 +372,8 @@ bool tc_shape(int dtype, int d, int P, int max_pages, int B, int Hq, int Hkv, in
   if (R > 128) return false;
   // chunk and slot numbers are 32-bit; a group's row tiles are of at least R rows
   if ((long long)B * Hq >= (1ll << 31)) return false;
-  const long long units = 2ll * B * Hkv + (long long)G * Hkv;   // costs are up to 11 a chunk
+  // and so are costs: up to 10 a chunk and 20 a unit, together 15 (chunks + 1) at most
+  const long long units = 2ll * B * Hkv + (long long)G * Hkv;
   return units * (((long long)max_pages * P + 127) / 128 + 1) < (1ll << 27);
 }
 }  // namespace

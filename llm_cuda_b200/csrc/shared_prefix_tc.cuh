@@ -25,8 +25,9 @@
 // across segments.  The issuer runs S two items ahead of P V.  Segments with up to 128 rows
 // have one item per chunk: their chunks alternate between the streams, and each stream
 // leaves a partial of its own.  Segments with 256 rows ("wide") have two items per chunk,
-// which halves the K/V traffic per row; tiles are wide when the work is long enough that
-// the coarser split does no harm (kLongChunks).
+// which halves the K/V traffic per row.  Tiles are wide when a group has more than 128 rows
+// (measured with narrow tiles against: 4 groups of 256 rows x 8192 tokens 78 us and 72, 256
+// rows x 512 tokens 24.9 and 23.2).
 //
 // The running maximum is only raised when it would grow by more than 8 (log2): weights up
 // to 2^8 are harmless in 16 bits, and O is then rarely rescaled.  Rounded to 16 bits: the
@@ -42,9 +43,6 @@ namespace tc {
 constexpr int kChunk = 128;        // tokens of a chunk (MMA N of S, K of P V)
 constexpr int kRing = 8;            // segments the producer may be ahead
 constexpr int kThreads = 384;      // two softmax warpgroups, one for the producer and the issuer
-
-// Wide tiles from this many 256-row chunks per CTA on.
-constexpr int kLongChunks = 6;
 
 struct TcParams {
   Params p;
@@ -103,22 +101,33 @@ __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, volatile int
 }
 
 // What the chunks cost, in units of some 450 cycles: a chunk of 128 rows at most 6 (K and V
-// of 64 KB at a fair share of the bandwidth are 2700 cycles), a chunk of a wide tile 11, and a
-// unit of own tokens 4 more, for the turn-over of a stream (fitted to the CTAs' end times).
-// With few chunks for the CTAs every chunk is 1.
-struct Costs {
-  int shared, own, unit;
-  __device__ __forceinline__ void set(int chunks, bool wide, int ctas) {
-    const bool few = chunks < 2 * ctas;   // otherwise a CTA's share exceeds any chunk's cost
-    shared = few ? 1 : wide ? 11 : 6;
-    own = few ? 1 : 6;
-    unit = few ? 0 : 4;
-  }
-  // where chunk j of an own unit begins, and the first chunk that begins at x or later
-  __device__ __forceinline__ int at(int j) const { return j ? unit + j * own : 0; }
+// of 64 KB at a fair share of the bandwidth are 2700 cycles), a chunk of a wide tile 10; a unit
+// 4 more, for the turn-over of a stream, and 1 per 16 rows that leave partials (fitted to the
+// CTAs' end times).  With few chunks for the CTAs every chunk is 1.
+struct Cost {
+  int chunk, unit;
+  // of a unit of n chunks: chunk j begins at j * chunk, the unit's own cost is behind the last
+  __device__ __forceinline__ int size(int n) const { return n ? n * chunk + unit : 0; }
+  // the first chunk that begins at x or later
   __device__ __forceinline__ int chunk_from(int x) const {
-    return x <= 0 ? 0 : max(1, quot(max(0, x - unit) + own - 1, own));
+    return x <= 0 ? 0 : quot(x + chunk - 1, chunk);
   }
+};
+struct Costs {
+  bool few;
+  int narrow;   // rows of a narrow tile
+  __device__ __forceinline__ void set(int chunks, int narrow_, int ctas) {
+    // Otherwise a CTA's share, 12 at least, exceeds any chunk's cost: no CTA between a unit's
+    // first and last one goes without a chunk of it (and leaves its slots unwritten).
+    few = chunks < 2 * ctas;
+    narrow = narrow_;
+  }
+  // of the units of a group with so many rows
+  __device__ __forceinline__ Cost shared(int rows) const {
+    if (few) return {1, 0};
+    return {rows > narrow ? 10 : 6, 4 + (min(rows, 2 * narrow) >> 4)};
+  }
+  __device__ __forceinline__ Cost own() const { return {few ? 1 : 6, few ? 0 : 4}; }
 };
 
 // How the total cost is dealt to C CTAs.
@@ -335,8 +344,8 @@ __device__ __forceinline__ int own_chunks(const Params& p, int s, int len) {
 }
 
 // Builds the tables with threads tid = 0 .. nt - 1 (whole warps; barrier 1).  totals: cost of
-// the shared units, of all, rows of a tile, chunks in all.  Inlined, so that tables in shared memory are
-// accessed as such.
+// the shared units, of all, rows of a tile, chunks in all.  Inlined, so that tables in shared
+// memory are accessed as such.
 __device__ __forceinline__ void bar1(int nt) { asm volatile("bar.sync 1, %0;" ::"r"(nt) : "memory"); }
 __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t, int* totals,
                                              int ctas, int tid, int nt) {
@@ -386,9 +395,9 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
     if (bad && lane == 0) atomicOr(p.status, kStatusBadGroup);
     const int narrow = tp.nb * p.R;
     const int per = (p.G + 31) >> 5, g0 = min(lane * per, p.G), g1 = min(g0 + per, p.G);
-    int w0 = 0, w1 = 0, u0 = 0, u1 = 0, most = 0;
+    int most = 0;
 #pragma unroll 1
-    for (int g = g0; g < g1; ++g) {   // a lane's groups with either tile
+    for (int g = g0; g < g1; ++g) {   // a lane's groups
       int n = 0, rows = 0;
       if (!bad && t.leader[g] != 0x7fffffff) {
         n = max(0, min(t.unit[g], t.s[g]));
@@ -396,18 +405,17 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
       }
       t.s[g] = n;
       t.rows[g] = rows;
-      if (n) {
-        const int ch = (n + kChunk - 1) / kChunk, ta = quot(rows + narrow - 1, narrow);
-        u0 += ta * p.Hkv;
-        u1 += (ta + 1) / 2 * p.Hkv;
-        w0 += ch * ta * p.Hkv;
-        w1 += ch * ((ta + 1) / 2) * p.Hkv;
-        most = max(most, rows);
-      }
+      if (n) most = max(most, rows);
     }
-    const bool wide = __reduce_max_sync(0xffffffffu, most) > narrow &&
-                      __reduce_add_sync(0xffffffffu, w1) >= kLongChunks * ctas;
+    const bool wide = __reduce_max_sync(0xffffffffu, most) > narrow;
     const int rt = wide ? 2 * narrow : narrow;
+    int chunks = 0, units = 0;
+#pragma unroll 1
+    for (int g = g0; g < g1; ++g) {
+      const int u = t.s[g] ? quot(t.rows[g] + rt - 1, rt) * p.Hkv : 0;
+      units += u;
+      chunks += u * ((t.s[g] + kChunk - 1) >> 7);
+    }
     // own chunks and units of this lane's sequences
     const int bper = (p.B + 31) >> 5, b0 = min(lane * bper, p.B), b1 = min(b0 + bper, p.B);
     __syncwarp();
@@ -420,12 +428,18 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
       oc += n * p.Hkv;
       ou += n ? p.Hkv : 0;
     }
-    const int chunks = __reduce_add_sync(0xffffffffu, (wide ? w1 : w0) + oc);
+    const int all = __reduce_add_sync(0xffffffffu, chunks + oc);
     Costs cost;
-    cost.set(chunks, wide, ctas);
-    const int wl = (wide ? w1 : w0) * cost.shared, ul = wide ? u1 : u0;
-    const int xl = oc * cost.own + ou * cost.unit;
-    int cs = wl, us = ul, xs = xl;
+    cost.set(all, narrow, ctas);
+    const Cost own = cost.own();
+    int wl = 0;
+#pragma unroll 1
+    for (int g = g0; g < g1; ++g)
+      if (t.s[g])
+        wl += quot(t.rows[g] + rt - 1, rt) * p.Hkv *
+              cost.shared(t.rows[g]).size((t.s[g] + kChunk - 1) >> 7);
+    const int xl = oc * own.chunk + ou * own.unit;
+    int cs = wl, us = units, xs = xl;
 #pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
       const int a = __shfl_up_sync(0xffffffffu, cs, o), b = __shfl_up_sync(0xffffffffu, us, o);
@@ -440,10 +454,10 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
       totals[0] = cs;
       totals[1] = cs + xs;
       totals[2] = rt;
-      totals[3] = chunks;
+      totals[3] = all;
     }
     cs -= wl;
-    us -= ul;
+    us -= units;
     xs -= xl;
 #pragma unroll 1
     for (int g = g0; g < g1; ++g) {
@@ -452,14 +466,14 @@ __device__ __forceinline__ void build_tables(const TcParams& tp, const Tables& t
       if (t.s[g]) {
         const int ta = quot(t.rows[g] + rt - 1, rt) * p.Hkv;
         us += ta;
-        cs += ta * ((t.s[g] + kChunk - 1) / kChunk) * cost.shared;
+        cs += ta * cost.shared(t.rows[g]).size((t.s[g] + kChunk - 1) >> 7);
       }
     }
 #pragma unroll 1
     for (int b = b0; b < b1; ++b) {
       t.own[b] = xs;
       const int gid = t.gid[b], n = own_chunks(p, gid >= 0 ? t.s[gid] : 0, t.len[b]);
-      xs += n ? (n * cost.own + cost.unit) * p.Hkv : 0;
+      xs += own.size(n) * p.Hkv;
     }
   }
   bar1(nt);
@@ -473,7 +487,7 @@ __device__ __noinline__ void write_plan(const TcParams& tp, const Tables& t, con
   Split split;
   split.set(totals[1], ctas);
   Costs cost;
-  cost.set(totals[3], rt > narrow, ctas);
+  cost.set(totals[3], narrow, ctas);
 #pragma unroll 1
   for (int e = first; e < p.B * p.Hkv; e += step) {
     const int b = quot(e, p.Hkv), hk = e - b * p.Hkv, g = t.gid[b];
@@ -485,17 +499,19 @@ __device__ __noinline__ void write_plan(const TcParams& tp, const Tables& t, con
       const int rr = (b - t.lo[g]) * p.R, tile = quot(rr, rt), u = hk * tiles + tile;
       const bool wide = min(rt, t.rows[g] - tile * rt) > narrow;
       const int q = wide && rr - tile * rt >= narrow ? 1 : 0;
-      const int x = t.start[g] + u * nch * cost.shared, a = split.owner(x);
-      const int segs = split.owner(x + (nch - 1) * cost.shared) - a + 1;
+      const Cost c = cost.shared(t.rows[g]);
+      const int x = t.start[g] + u * c.size(nch), a = split.owner(x);
+      const int segs = split.owner(x + (nch - 1) * c.chunk) - a + 1;
       v.x = 2 * (t.unit[g] + u + a) + q;
       v.z = (wide ? segs : 2 * segs) | (rr - tile * rt - q * narrow) << 16 |
             (wide ? (int)0x80000000 : 0);
     }
     const int nch = own_chunks(p, s, t.len[b]);
     if (nch) {
-      const int x = totals[0] + t.own[b] + hk * (nch * cost.own + cost.unit), a = split.owner(x);
+      const Cost c = cost.own();
+      const int x = totals[0] + t.own[b] + hk * c.size(nch), a = split.owner(x);
       v.y = 2 * (e + a);
-      v.w = 2 * (split.owner(x + cost.at(nch - 1)) - a + 1);
+      v.w = 2 * (split.owner(x + (nch - 1) * c.chunk) - a + 1);
     }
     tp.plan[e] = v;
   }
@@ -549,7 +565,7 @@ struct Walker {
     const Params& p = tp.p;
     X0 = totals[0];
     rt = totals[2];
-    cost.set(totals[3], rt > tp.nb * p.R, gridDim.x);
+    cost.set(totals[3], tp.nb * p.R, gridDim.x);
     Split split;
     split.set(totals[1], gridDim.x);
     const bool idle = (int)blockIdx.x >= split.C;
@@ -565,17 +581,19 @@ struct Walker {
       int j0, j1;
       if (x < X0) {
         int nch, tiles, size;
+        Cost c;
 #pragma unroll 1
         while (true) {   // the group that holds x
           nch = (t.s[g] + kChunk - 1) / kChunk;
           tiles = quot(t.rows[g] + rt - 1, rt);
-          size = nch * cost.shared;
+          c = cost.shared(t.rows[g]);
+          size = c.size(nch);
           if (x < t.start[g] + size * tiles * p.Hkv || g + 1 >= p.G) break;
           ++g;
         }
         const int y = x - t.start[g], ul = quot(y, size), base = x - (y - ul * size);
-        j0 = quot(x - base + cost.shared - 1, cost.shared);
-        j1 = min(nch, quot(x1 - base + cost.shared - 1, cost.shared));
+        j0 = c.chunk_from(x - base);
+        j1 = min(nch, c.chunk_from(x1 - base));
         x = min(x1, base + size);
         sg.hk = quot(ul, tiles);
         const int tile = ul - sg.hk * tiles;
@@ -589,18 +607,19 @@ struct Walker {
         sg.hi = t.s[g];
         sg.slot = 2 * (t.unit[g] + ul + (int)blockIdx.x);
       } else {
+        const Cost c = cost.own();
         int nch, s, size;
 #pragma unroll 1
         while (true) {   // the sequence that holds x
           s = t.gid[b] >= 0 ? t.s[t.gid[b]] : 0;
           nch = own_chunks(p, s, t.len[b]);
-          size = nch ? nch * cost.own + cost.unit : 0;
+          size = c.size(nch);
           if (x - X0 < t.own[b] + size * p.Hkv || b + 1 >= p.B) break;
           ++b;
         }
         const int y = x - X0 - t.own[b], hk = quot(y, size), base = x - (y - hk * size);
-        j0 = cost.chunk_from(x - base);
-        j1 = min(nch, cost.chunk_from(x1 - base));
+        j0 = c.chunk_from(x - base);
+        j1 = min(nch, c.chunk_from(x1 - base));
         x = min(x1, base + size);
         sg.own = 1;
         sg.hk = hk;
@@ -828,8 +847,7 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         load(c, last);
       }
     };
-    // 32-token blocks of the current chunk that hold tokens
-    auto blocks = [](const Cursor& c) { return (min(kChunk, c.hi - c.t0 - c.j * kChunk) + 31) >> 5; };
+    auto tokens = [](const Cursor& c) { return min(kChunk, c.hi - c.t0 - c.j * kChunk); };
     // V: 16 tokens of a k-step are inside a box, or two boxes of 8 (descriptor units of 16 B)
     const int vbox = min(p.P, kChunk), vsh = 31 - __clz(vbox), vstep = vbox * 8 * S::kHalves;
     Cursor a = {}, b = {};     // S (a) runs two items ahead of P V (b)
@@ -847,7 +865,7 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         fence_after();
         const uint64_t vd = desc_mnmajor(sb + S::kV + st * S::kOperand, vbox);
         const bool first = b.wide ? b.j == 0 : b.j < 2;
-        const int steps = 2 * blocks(b);
+        const int steps = (tokens(b) + 15) >> 4;
 #pragma unroll
         for (int kk = 0; kk < kChunk / 16; ++kk) {
           if (kk >= steps) continue;
@@ -867,7 +885,7 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         fence_after();
         const uint64_t qd = desc_kmajor(sb + S::kQ + qb * S::kOperand);
         const uint64_t kd = desc_kmajor(sb + S::kK + st * S::kOperand);
-        const uint32_t id = ID_S | ((uint32_t)(blocks(a) * 4) << 17);   // N = 32 per block
+        const uint32_t id = ID_S | ((uint32_t)((tokens(a) + 31) >> 5 << 2) << 17);   // N = 32, 64 ...
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t off = ((kk / 4) * S::kTile + (kk % 4) * 32) >> 4;
@@ -936,9 +954,11 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             for (int x = 0; x < ((hi + 63) & ~63); x += 16) {
               if (x >= lo && x + 16 <= hi) continue;
               uint32_t o[16];
-              ld16(ts + x, o);
-              wait_ld();
-              landed(o);
+              if (x < hi && x + 16 > lo) {
+                ld16(ts + x, o);
+                wait_ld();
+                landed(o);
+              }
 #pragma unroll
               for (int e = 0; e < 16; ++e)
                 if (x + e < lo || x + e >= hi) o[e] = __float_as_uint(kNegInf);
@@ -1009,14 +1029,15 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
           wait_st();
         }
         if (real) {
-          if (hi < 32 * nb && (!sg.wide || q == 0)) {
+          const int end = (hi + 15) & ~15;     // of P V's last step
+          if (hi < end && (!sg.wide || q == 0)) {
             // Rows of V behind the last token hold anything; a weight 0 would not silence a
             // NaN.  S of this item follows the products of the stream's item before, so the
             // stage's earlier chunk is done: this wait cannot take its phase for the chunk's.
             const int st = (k + j) % NS;
             wait(vfull + 8 * st, ((k + j) / NS) & 1, abort_flag, p.status);
             const uint32_t v0 = sb + S::kV + st * S::kOperand;
-            const int per = (32 * nb - hi) * 8;
+            const int per = (end - hi) * 8;
 #pragma unroll 1
             for (int i = r; i < per * S::kHalves; i += 128) {
               const int h = i >= per ? 1 : 0, w = i - h * per, tok = hi + (w >> 3);
