@@ -214,8 +214,10 @@ __global__ void __launch_bounds__(kThreads) units_kernel(const Params p, int gro
   pdl_launch_dependents();
   pdl_wait();
 
+  const bool ok = groups_ok(p);
   int t_begin, t_end;
   if (u.group) {
+    if (!ok) return;
     const int g = unit / group_tiles, tile = unit % group_tiles;
     int hi, s, leader;
     group_range(p, g, u.lo, hi);
@@ -231,7 +233,7 @@ __global__ void __launch_bounds__(kThreads) units_kernel(const Params p, int gro
     u.lo = unit / seq_tiles;
     u.row0 = (unit % seq_tiles) * 16;
     u.nrows = p.R;
-    const int g = group_of(p, u.lo, scratch);
+    const int g = ok ? group_of(p, u.lo, scratch) : -1;
     int s = 0;
     if (g >= 0) {
       int glo, ghi, leader;

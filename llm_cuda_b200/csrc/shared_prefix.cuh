@@ -44,14 +44,23 @@ __device__ __forceinline__ int seq_len(const Params& p, int b, bool report) {
   return n;
 }
 
-// Range of group g, clamped to the batch and to max_group sequences.
+// Whether every group is a range of the batch, by all threads of the block.  If not, nothing is
+// shared: the ranges may overlap.
+__device__ __forceinline__ bool groups_ok(const Params& p) {
+  int bad = 0;
+  for (int g = threadIdx.x; g < p.G; g += blockDim.x) {
+    const int lo = p.starts[g], hi = p.starts[g + 1];
+    bad |= lo < 0 || hi < lo || hi > p.B;
+  }
+  bad = __syncthreads_or(bad);
+  if (bad && threadIdx.x == 0) atomicOr(p.status, kStatusBadGroup);
+  return !bad;
+}
+
+// Range of group g, clamped to max_group sequences.
 __device__ __forceinline__ void group_range(const Params& p, int g, int& lo, int& hi) {
   lo = p.starts[g];
   hi = p.starts[g + 1];
-  if (lo < 0 || hi < lo || hi > p.B) {
-    atomicOr(p.status, kStatusBadGroup);
-    lo = hi = 0;
-  }
   if (hi - lo > p.max_group) hi = lo + p.max_group;
 }
 
@@ -92,7 +101,7 @@ __device__ __forceinline__ int group_of(const Params& p, int b, int* scratch) {
   __syncthreads();
   for (int g = threadIdx.x; g < p.G; g += blockDim.x) {
     const int lo = p.starts[g], hi = p.starts[g + 1];
-    if (lo >= 0 && hi <= p.B && b >= lo && b < hi && b - lo < p.max_group) atomicMax(scratch, g);
+    if (b >= lo && b < hi && b - lo < p.max_group) atomicMax(scratch, g);
   }
   __syncthreads();
   const int g = *scratch;

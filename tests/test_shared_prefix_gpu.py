@@ -260,12 +260,41 @@ def test_captured_graph_follows_lengths_and_two_graphs_overlap():
             b.shared_lens.copy_(torch.tensor([min(290, min(lens))], dtype=torch.int32))
 
 
+@pytest.mark.parametrize("force_generic", [False, True])
+def test_pages_behind_2_31_elements(force_generic):
+    """The same pages at the end of a pool of more than 2^31 elements: the same bits."""
+    b = Batch([3], [200], [210, 300, 251], 8, 2, 128, 64, BF, seed=13)
+    want = b.run(force_generic=force_generic)
+    n = b.kp.shape[0]
+    first = 2 ** 31 // b.kp[0].numel() + 1
+    for name in ("kp", "vp"):
+        small = getattr(b, name)
+        pool = torch.empty(first + n, *small.shape[1:], dtype=BF, device=DEV)
+        pool[first:] = small
+        setattr(b, name, pool)
+    b.bt = torch.where(b.bt >= 0, b.bt + first, b.bt)
+    assert torch.equal(b.run(force_generic=force_generic), want)
+
+
 def test_same_inputs_same_bits():
     b = Batch([20, 3], [900, 90], [901 + i for i in range(20)] + [90, 91, 99], 32, 8, 128, 16, BF,
               seed=11)
     first = b.run()
     for _ in range(3):
         assert torch.equal(b.run(), first)
+
+
+@pytest.mark.parametrize("force_generic", [False, True])
+@pytest.mark.parametrize("starts", [[0, 3, 1, 4], [0, 2, 3, 9], [-1, 2, 3, 4], [3, 0, 4, 2]])
+def test_bad_groups_share_nothing(starts, force_generic):
+    """One range that is none: the status word, and every sequence reads its own context."""
+    b = Batch([2, 1, 1], [64, 64, 64], [70, 80, 90, 65], 8, 2, 128, 16, BF, seed=12)
+    b.starts.copy_(torch.tensor(starts, dtype=torch.int32))
+    out = b.run(force_generic=force_generic)
+    with pytest.raises(N.DeviceStatusError, match="groups"):
+        N.raise_on_status(b.status)
+    b.status.zero_()
+    b.check(out)
 
 
 def test_bad_inputs_set_the_status_word():
