@@ -51,7 +51,7 @@ __device__ __forceinline__ void attend(const Params& p, const Unit& u, float* sm
   float* Ps = Vs + kTok * DP;     // [ROWS][PS]
   const int d = p.d, tid = threadIdx.x, rg = tid >> 4, c = tid & 15;
   const T* q = reinterpret_cast<const T*>(p.q);
-  for (int i = tid; i < ROWS * DP; i += kThreads) {
+  for (int i = u.first < u.last ? tid : ROWS * DP; i < ROWS * DP; i += kThreads) {
     const int r = i / DP, col = i - r * DP, row = u.row0 + r;
     float v = 0.f;
     if (row < u.nrows && col < d) {
@@ -76,42 +76,73 @@ __device__ __forceinline__ void attend(const Params& p, const Unit& u, float* sm
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[r][j][e] = 0.f;
   }
+  // 8 threads per token bring its key and value; columns from d on are zero.  A step's vectors
+  // are on their way while the step before is computed, its page numbers a step earlier still
+  // (10 sequences of up to 25000 tokens at 4 fp32 KV heads of 64: 234 us, fetched when needed
+  // 259 us; 383 us when warps without a row computed too).
+  constexpr int NV = DP / (8 * VEC);
+  constexpr bool kAhead = RPT == 1 && NV <= 4;  // beyond that the registers cost more
+  const int t = tid >> 3, part = tid & 7;
+  uint4 kr[NV], vr[NV];
+  const int32_t* table = p.block_table + (long long)u.table_row * p.max_pages;
+  auto page_at = [&](int t0) { return t0 + t < u.last ? table[(t0 + t) / p.P] : 0; };
+  auto offset = [&](int t0, int page) -> long long {
+    if (page < 0 || page >= p.num_pages) {
+      atomicOr(p.status, kStatusBadPage);
+      page = 0;
+    }
+    return (((long long)page * p.Hkv + u.hk) * p.P + (t0 + t) % p.P) * d;
+  };
+  auto fetch = [&](int t0, int page) {
+    const bool have = t0 + t < u.last;
+    const long long base = have ? offset(t0, page) : 0;
+#pragma unroll
+    for (int n = 0; n < NV; ++n) {
+      const int i = (part + 8 * n) * VEC;
+      const bool in = have && i < d;
+      kr[n] = in ? __ldg(reinterpret_cast<const uint4*>(kp + base + i)) : make_uint4(0u, 0u, 0u, 0u);
+      vr[n] = in ? __ldg(reinterpret_cast<const uint4*>(vp + base + i)) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  const bool live = u.row0 + (tid >> 5) * 2 * RPT < u.nrows;   // does this warp have a row?
+  int page = page_at(u.first);
+  if (vec && kAhead) {
+    fetch(u.first, page);
+    page = page_at(u.first + kTok);
+  }
   for (int t0 = u.first; t0 < u.last; t0 += kTok) {
     const int nt = min(kTok, u.last - t0);
     __syncthreads();
-    {   // 8 threads per token bring its key and value; columns from d on are zero
-      const int t = tid >> 3, part = tid & 7;
-      const bool have = t < nt;
-      long long base = 0;
-      if (have) {
-        const int tok = t0 + t;
-        base = (((long long)page_of(p, u.table_row, tok) * p.Hkv + u.hk) * p.P + tok % p.P) * d;
+    if (vec) {
+      if (!kAhead) fetch(t0, page);
+#pragma unroll
+      for (int n = 0; n < NV; ++n) {
+        const int i = (part + 8 * n) * VEC;
+        const T* ke = reinterpret_cast<const T*>(&kr[n]);
+        const T* ve = reinterpret_cast<const T*>(&vr[n]);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          Ks[t * QS + i + e] = to_f32(ke[e]);
+          Vs[t * DP + i + e] = to_f32(ve[e]);
+        }
       }
-      if (vec) {
-#pragma unroll
-        for (int i = part * VEC; i < DP; i += 8 * VEC) {
-          uint4 kv = make_uint4(0u, 0u, 0u, 0u), vv = kv;
-          if (have && i < d) {
-            kv = __ldg(reinterpret_cast<const uint4*>(kp + base + i));
-            vv = __ldg(reinterpret_cast<const uint4*>(vp + base + i));
-          }
-          const T* ke = reinterpret_cast<const T*>(&kv);
-          const T* ve = reinterpret_cast<const T*>(&vv);
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            Ks[t * QS + i + e] = to_f32(ke[e]);
-            Vs[t * DP + i + e] = to_f32(ve[e]);
-          }
-        }
-      } else {
-        for (int i = part; i < DP; i += 8) {
-          const bool in = have && i < d;
-          Ks[t * QS + i] = in ? to_f32(kp[base + i]) : 0.f;
-          Vs[t * DP + i] = in ? to_f32(vp[base + i]) : 0.f;
-        }
+    } else {
+      const bool have = t < nt;
+      const long long base = have ? offset(t0, page) : 0;
+      for (int i = part; i < DP; i += 8) {
+        const bool in = have && i < d;
+        Ks[t * QS + i] = in ? to_f32(kp[base + i]) : 0.f;
+        Vs[t * DP + i] = in ? to_f32(vp[base + i]) : 0.f;
       }
     }
     __syncthreads();
+    if (vec && kAhead) {
+      fetch(t0 + kTok, page);
+      page = page_at(t0 + 2 * kTok);
+    } else {
+      page = page_at(t0 + kTok);
+    }
+    if (!live) continue;
     float x0[RPT], x1[RPT];
 #pragma unroll
     for (int r = 0; r < RPT; ++r) x0[r] = x1[r] = 0.f;
@@ -199,8 +230,10 @@ __device__ __forceinline__ void attend(const Params& p, const Unit& u, float* sm
 // slots below split_g are the shared part's, the others the own part's.
 // Grid: x = unit of a KV head and split, y = KV head.  Units: the tiles of the groups' rows
 // (16 * rpt rows; sized for max_group), then the 16-row tiles of every sequence.
+// Three blocks per SM, for a few spilled words, up to head size 128 (16 groups of 48 rows x 130 tokens at 8 fp32 KV
+// heads of 128: 70.7 us, left to the compiler two and 77.3 us).
 template <typename T, int NJ>
-__global__ void __launch_bounds__(kThreads) units_kernel(const Params p, int group_tiles,
+__global__ void __launch_bounds__(kThreads, NJ <= 2 ? 3 : 1) units_kernel(const Params p, int group_tiles,
                                                          int seq_tiles, int rpt) {
   extern __shared__ __align__(16) float sm[];
   __shared__ int scratch[2];

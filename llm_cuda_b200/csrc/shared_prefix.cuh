@@ -109,15 +109,5 @@ __device__ __forceinline__ int group_of(const Params& p, int b, int* scratch) {
   return g;
 }
 
-// Physical page of a sequence's token, 0 and a status bit for a bad table entry.
-__device__ __forceinline__ int page_of(const Params& p, int b, int tok) {
-  const int page = p.block_table[(long long)b * p.max_pages + tok / p.P];
-  if (page < 0 || page >= p.num_pages) {
-    atomicOr(p.status, kStatusBadPage);
-    return 0;
-  }
-  return page;
-}
-
 }  // namespace prefix
 }  // namespace llmc
