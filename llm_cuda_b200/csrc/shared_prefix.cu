@@ -230,8 +230,8 @@ __device__ __forceinline__ void attend(const Params& p, const Unit& u, float* sm
 // slots below split_g are the shared part's, the others the own part's.
 // Grid: x = unit of a KV head and split, y = KV head.  Units: the tiles of the groups' rows
 // (16 * rpt rows; sized for max_group), then the 16-row tiles of every sequence.
-// Three blocks per SM, for a few spilled words, up to head size 128 (16 groups of 48 rows x 130 tokens at 8 fp32 KV
-// heads of 128: 70.7 us, left to the compiler two and 77.3 us).
+// Three blocks per SM, for a few spilled words, up to head size 128 (16 groups of 48 rows x 130
+// tokens at 8 fp32 KV heads of 128: 70.6 us, left to the compiler two and 77.3 us).
 template <typename T, int NJ>
 __global__ void __launch_bounds__(kThreads, NJ <= 2 ? 3 : 1) units_kernel(const Params p, int group_tiles,
                                                          int seq_tiles, int rpt) {
