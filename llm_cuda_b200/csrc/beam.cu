@@ -128,20 +128,6 @@ __device__ __forceinline__ void top_compact(WarpTop& t, int lane) {
   }
 }
 
-// The n-th largest of the lanes' values (n <= 32): a bitonic sort across the warp.
-__device__ __forceinline__ float nth_lane_max(float v, int n, int lane) {
-#pragma unroll
-  for (int k = 2; k <= 32; k <<= 1) {
-#pragma unroll
-    for (int j = k >> 1; j; j >>= 1) {
-      const float o = __shfl_xor_sync(0xffffffffu, v, j);
-      const bool up = ((lane & k) == 0) == ((lane & j) == 0);   // descending
-      v = up ? fmaxf(v, o) : fminf(v, o);
-    }
-  }
-  return __shfl_sync(0xffffffffu, v, n - 1);
-}
-
 // 2^x by the hardware (2 ulp); exp2f adds a range check for results below 2^-126, which
 // a sum whose largest term is 1 does not notice.
 __device__ __forceinline__ float ex2(float x) {
