@@ -14,8 +14,8 @@
 // CTA fetches the tasks' lists and sums through distributed shared memory and ranks the
 // candidates by their scores in the same way.
 // Bound: the logits are read once from HBM; then the exponentials (16 a cycle and SM).
-// Measured before the cells, with lists kept up to date while streaming: 104 us for 131 MB
-// of logits, of which the exponentials were a fifth.
+// Measured on 64 prompts of 8 beams, 131 MB of bf16 logits: 41 us (floor 20 us), some 29 of
+// them the stream; with lists kept up to date while streaming instead of cells 104 us.
 //
 // Sums of exponentials are held in fp32 per thread, joined in fp32 inside a split and in
 // fp64 across splits; scores are ranked in fp64 (candidates of different beams are often
@@ -674,8 +674,8 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
 //
 // The copies of a prompt form a permutation with repeats, in place: a thread loads one
 // 16-byte vector of all K pages, then stores them, so no copy sees another's result.  The
-// table is moved the same way, a thread per column.  Bound: HBM (the moved tokens), and
-// at small sizes the launch.
+// table is moved the same way, a thread per column.  Bound: HBM (the moved tokens; 112.5 us
+// for 638 MB, 87% of a plain copy's rate), and at small sizes the launch (2.9 us).
 struct ReorderParams {
   uint8_t* pools;              // [layers][2][num_pages][Hkv][P][d]
   const int32_t* own_table;    // [G * K, max_pages]

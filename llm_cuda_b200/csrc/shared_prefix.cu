@@ -16,6 +16,8 @@
 // units of 16 or 64 query rows x a range of tokens, in fp32 on the CUDA cores, with 32
 // tokens of K and V at a time in shared memory.  Bound: the FMA pipes and, as evenly, the
 // shared-memory reads that feed them (4 rows x 2 tokens or 4 rows x 4 columns a thread).
+// Measured in fp32: 25 us for 1.7 MB (launches and dependent loads), 233 us for 408 MB of K and
+// V with 4 query rows per KV head (1.75 TB/s).
 #include <climits>
 #include <string>
 
