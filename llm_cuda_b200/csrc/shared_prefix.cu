@@ -16,8 +16,8 @@
 // units of 16 or 64 query rows x a range of tokens, in fp32 on the CUDA cores, with 32
 // tokens of K and V at a time in shared memory.  Bound: the FMA pipes and, as evenly, the
 // shared-memory reads that feed them (4 rows x 2 tokens or 4 rows x 4 columns a thread).
-// Measured in fp32: 25 us for 1.7 MB (launches and dependent loads), 233 us for 408 MB of K and
-// V with 4 query rows per KV head (1.75 TB/s).
+// Measured in fp32: 24 us for 1.7 MB (launches and dependent loads), 230 us for 408 MB of K and
+// V with 4 query rows per KV head (1.8 TB/s).
 #include <climits>
 #include <string>
 
@@ -228,17 +228,53 @@ __device__ __forceinline__ void attend(const Params& p, const Unit& u, float* sm
   }
 }
 
+// What the blocks have to know of the groups, once for all of them: groups[g] = {first
+// sequence, end, shared tokens, leader (-1: all empty)}, and the shared tokens of every
+// sequence.  One block: a warp per group.  (16 groups of 48 rows x 130 fp32 tokens: 68.0 us,
+// with every block of units_kernel finding out for itself 70.6; the smallest case 24.0, 24.8.)
+__global__ void __launch_bounds__(1024) groups_kernel(const Params p, int4* groups, int* seq_s) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  // One bad range and nothing is shared: the ranges may overlap.
+  int bad = 0;
+  for (int g = threadIdx.x; g < p.G; g += blockDim.x) {
+    const int lo = p.starts[g], hi = p.starts[g + 1];
+    bad |= lo < 0 || hi < lo || hi > p.B;
+  }
+  for (int b = threadIdx.x; b < p.B; b += blockDim.x) seq_s[b] = 0;
+  bad = __syncthreads_or(bad);
+  if (bad && threadIdx.x == 0) atomicOr(p.status, kStatusBadGroup);
+  for (int g = threadIdx.x >> 5; g < p.G; g += blockDim.x >> 5) {
+    const int lo = bad ? 0 : p.starts[g];
+    const int hi = bad ? 0 : min(p.starts[g + 1], lo + min(p.max_group, p.B - lo));
+    int mn = INT_MAX, first = INT_MAX;
+    for (int b = lo + lane; b < hi; b += 32) {
+      const int n = seq_len(p, b, false);
+      if (n > 0) {
+        mn = min(mn, n);
+        first = min(first, b);
+      }
+    }
+    mn = __reduce_min_sync(0xffffffffu, mn);
+    first = __reduce_min_sync(0xffffffffu, first);
+    const int s = first == INT_MAX ? 0 : max(0, min(p.shared[g], mn));
+    if (lane == 0) groups[g] = make_int4(lo, hi, s, first == INT_MAX ? -1 : first);
+    if (s)
+      for (int b = lo + lane; b < hi; b += 32) seq_s[b] = s;
+  }
+}
+
 // Partials: part_o [split_g + split_o][B * Hq][d], part_lse [split_g + split_o][B * Hq];
 // slots below split_g are the shared part's, the others the own part's.
 // Grid: x = unit of a KV head and split, y = KV head.  Units: the tiles of the groups' rows
 // (16 * rpt rows; sized for max_group), then the 16-row tiles of every sequence.
 // Three blocks per SM, for a few spilled words, up to head size 128 (16 groups of 48 rows x 130
-// tokens at 8 fp32 KV heads of 128: 70.6 us, left to the compiler two and 77.3 us).
+// tokens at 8 fp32 KV heads of 128: 70.6 us, with two, as the compiler leaves it, 77.3 us).
 template <typename T, int NJ>
-__global__ void __launch_bounds__(kThreads, NJ <= 2 ? 3 : 1) units_kernel(const Params p, int group_tiles,
-                                                         int seq_tiles, int rpt) {
+__global__ void __launch_bounds__(kThreads, NJ <= 2 ? 3 : 1) units_kernel(
+    const Params p, const int4* groups, const int* seq_s, int group_tiles, int seq_tiles, int rpt) {
   extern __shared__ __align__(16) float sm[];
-  __shared__ int scratch[2];
   const int of_groups = p.G * group_tiles * p.split_g;
   Unit u;
   u.hk = blockIdx.y;
@@ -249,34 +285,23 @@ __global__ void __launch_bounds__(kThreads, NJ <= 2 ? 3 : 1) units_kernel(const 
   pdl_launch_dependents();
   pdl_wait();
 
-  const bool ok = groups_ok(p);
   int t_begin, t_end;
   if (u.group) {
-    if (!ok) return;
-    const int g = unit / group_tiles, tile = unit % group_tiles;
-    int hi, s, leader;
-    group_range(p, g, u.lo, hi);
-    u.row0 = tile * 16 * rpt;
-    u.nrows = (hi - u.lo) * p.R;
-    if (u.row0 >= u.nrows) return;
-    group_prefix(p, g, u.lo, hi, scratch, s, leader);
-    if (s == 0) return;            // the sequences' own units mark the shared slots empty
+    const int4 g = groups[unit / group_tiles];
+    u.lo = g.x;
+    u.row0 = unit % group_tiles * 16 * rpt;
+    u.nrows = (g.y - g.x) * p.R;
+    // without shared tokens the sequences' own units mark the shared slots empty
+    if (u.row0 >= u.nrows || g.z == 0) return;
     t_begin = 0;
-    t_end = s;
-    u.table_row = leader;
+    t_end = g.z;
+    u.table_row = g.w;
   } else {
     u.lo = unit / seq_tiles;
     u.row0 = (unit % seq_tiles) * 16;
     u.nrows = p.R;
-    const int g = ok ? group_of(p, u.lo, scratch) : -1;
-    int s = 0;
-    if (g >= 0) {
-      int glo, ghi, leader;
-      group_range(p, g, glo, ghi);
-      group_prefix(p, g, glo, ghi, scratch, s, leader);
-    }
     t_end = seq_len(p, u.lo, split == 0 && threadIdx.x == 0);
-    t_begin = min(s, t_end);
+    t_begin = min(seq_s[u.lo], t_end);
     u.table_row = u.lo;
     if (t_begin == 0 && split == 0)   // no shared part
       for (int i = threadIdx.x; i < 16 * p.split_g; i += kThreads)
@@ -371,9 +396,14 @@ GenericPlan generic_plan(int B, int Hq, int Hkv, int G, int max_group) {
   return z;
 }
 
+size_t generic_tables(int B, int G) {   // groups_kernel's, in front of the partials
+  return ((size_t)G * sizeof(int4) + (size_t)B * sizeof(int) + 15) / 16 * 16;
+}
+
 size_t generic_workspace(int B, int Hq, int Hkv, int d, int G, int max_group) {
   const GenericPlan z = generic_plan(B, Hq, Hkv, G, max_group);
-  return (size_t)(z.split_g + z.split_o) * B * Hq * ((size_t)d + 1) * sizeof(float);
+  return (size_t)(z.split_g + z.split_o) * B * Hq * ((size_t)d + 1) * sizeof(float) +
+         generic_tables(B, G);
 }
 
 // Workspace of the tensor-core kernels: plan, tables (if they do not fit shared memory),
@@ -454,18 +484,23 @@ static cudaError_t launch_generic_d(prefix::Params p, float* ws, std::string* er
   const GenericPlan z = generic_plan(p.B, p.Hq, p.Hkv, p.G, p.max_group);
   p.split_g = z.split_g;
   p.split_o = z.split_o;
-  p.part_o = ws;
-  p.part_lse = ws + (size_t)(z.split_g + z.split_o) * p.B * p.Hq * p.d;
+  int4* groups = reinterpret_cast<int4*>(ws);
+  int* seq_s = reinterpret_cast<int*>(groups + p.G);
+  p.part_o = ws + generic_tables(p.B, p.G) / sizeof(float);
+  p.part_lse = p.part_o + (size_t)(z.split_g + z.split_o) * p.B * p.Hq * p.d;
   const long long blocks = (long long)p.G * z.group_tiles * z.split_g +
                            (long long)p.B * z.seq_tiles * z.split_o;
   if (blocks > INT_MAX || p.Hkv > 65535) {
     *err = "too many row tiles (groups x max_group, sequences) for this shape";
     return cudaErrorInvalidConfiguration;
   }
-  cudaError_t e = launch_chained<gen::units_kernel<T, NJ>>(
+  cudaError_t e = launch_chained<gen::groups_kernel>(dim3(1), dim3(1024), 0, stream, p, groups,
+                                                     seq_s);
+  if (e != cudaSuccess) return e;
+  e = launch_chained<gen::units_kernel<T, NJ>>(
       dim3((unsigned)blocks, p.Hkv), dim3(gen::kThreads),
-      gen::smem_floats(z.rpt, 64 * NJ) * sizeof(float), stream, p, z.group_tiles, z.seq_tiles,
-      z.rpt);
+      gen::smem_floats(z.rpt, 64 * NJ) * sizeof(float), stream, p, groups, seq_s, z.group_tiles,
+      z.seq_tiles, z.rpt);
   if (e != cudaSuccess) return e;
   const long long rows = (long long)p.B * p.Hq;
   return launch_chained<gen::join_kernel<T>>(dim3((unsigned)((rows + 7) / 8)), dim3(256), 0,
