@@ -166,11 +166,11 @@ __device__ __forceinline__ uint64_t desc_kmajor(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) |
          (2ull << 61);
 }
-__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr, int box) {
+__device__ __forceinline__ uint64_t desc_mnmajor(uint32_t addr, int box, int halves) {
   // 128-byte swizzle, 64 contiguous N elements per row (a token), laid out [box][half][rows]:
-  // the other 64 N elements are a box's rows further (leading offset), the next 8 tokens
-  // follow (stride offset) unless a box holds only 8.
-  const uint32_t lead = (uint32_t)box * 128, stride = box == 8 ? 2 * lead : 1024u;
+  // the other 64 N elements are a box's rows further (leading offset; unused with one half),
+  // the next 8 tokens follow (stride offset), behind the other half if a box holds only 8.
+  const uint32_t lead = (uint32_t)box * 128, stride = box == 8 ? halves * lead : 1024u;
   return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lead >> 4) << 16) |
          ((uint64_t)(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
@@ -868,7 +868,7 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
         wait(pready + 8 * s, (ready >> s) & 1, abort_flag, p.status);
         if (b.sub == 0) wait(vfull + 8 * st, (b.k / NS) & 1, abort_flag, p.status);
         fence_after();
-        const uint64_t vd = desc_mnmajor(sb + S::kV + st * S::kOperand, vbox);
+        const uint64_t vd = desc_mnmajor(sb + S::kV + st * S::kOperand, vbox, S::kHalves);
         const bool first = b.wide ? b.j == 0 : b.j < 2;
         const int steps = (tokens(b) + 15) >> 4;
 #pragma unroll

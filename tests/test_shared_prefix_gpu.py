@@ -383,3 +383,16 @@ def test_batch_whose_tables_do_not_fit_shared_memory():
     lens = [shared[g] + (3 * g + j) % 9 for g, n in enumerate(sizes) for j in range(n)]
     b = Batch(sizes, shared, lens, 2, 1, 128, 16, BF, seed=15)
     b.check(b.run(max_group=5))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("P", [8, 16, 32, 64, 128, 256, 384])
+def test_every_page_size_of_the_tensor_cores(P, d, dtype):
+    """Shared and own parts of several chunks with odd ends, narrow tiles and (the last group,
+    of 70 x 2 rows per KV head) wide ones; pages of 8 tokens at head size 64 among them, whose V
+    boxes lie closer together than those of two halves."""
+    b = Batch([3, 2, 70], [300, 8, 133],
+              [301, 463, 700, 9, 330] + [133 + (5 * i) % 37 for i in range(70)], 8, 4, d, P, dtype,
+              seed=P + d)
+    b.check(b.run())
