@@ -147,9 +147,9 @@ __device__ __forceinline__ float2 unpair(uint64_t v) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
   return r;
 }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
@@ -297,9 +297,11 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
                       (size_t)tasks * (n + 1) + kCells * kThreads / 2;
   Cand* cand = reinterpret_cast<Cand*>(wbuf + keys + (keys & 1));
   Cand* half = cand + (size_t)tasks * n;
-  double* row_lse = reinterpret_cast<double*>(half + spare_cands(n, tasks));
-  double* row_b = row_lse + K;
-  int* row_kind = reinterpret_cast<int*>(row_b + K);            // 0 live, 1 dead, 2 finished
+  // of a row: log-sum-exp = row_max + row_log, beam score, 0 live, 1 dead, 2 finished
+  double* row_log = reinterpret_cast<double*>(half + spare_cands(n, tasks));
+  double* row_b = row_log + K;
+  float* row_max = reinterpret_cast<float*>(row_b + K);
+  int* row_kind = reinterpret_cast<int*>(row_max + K);
   __shared__ float red_m[kWarps], red_s[kWarps], red_b[kWarps];
   __shared__ __align__(16) float maxima[kThreads / 2];
   __shared__ int hits[kThreads];
@@ -358,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
       }
     };
     // One pass: maximum, sum, cells.
-    float m = kNegInf, ml = 0.f;     // ml = m log2(e), rounded; 0 while m = -inf
+    float m = kNegInf, ref = 0.f;    // ref = m; 0 while m = -inf
     uint64_t s2 = pair(0.f, 0.f);
     // tiles of a cell, the same for all warps
     const int tiles = ((v1 - v0 + kWarps - 1) / kWarps + 32 * kU - 1) / (32 * kU);
@@ -383,21 +385,20 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
         in_cell = 0;
         ++cell;
       }
-      // The exponent x log2(e) - ml is one fused operation; ml's rounding is common to all
-      // terms and taken out at the end.
+      // Exponents are (x - m) log2(e), the difference first: never positive, and 0 at the
+      // maximum, for logits of any size (finite masks up to the type's lowest value).
       if (tile_m > m) {
-        const float nl = tile_m * kLog2e, f = ex2(ml - nl);
+        const float f = ex2((m - tile_m) * kLog2e);
         const float2 o = unpair(s2);
-        s2 = m == kNegInf ? s2 : pair(o.x * f, o.y * f);
-        m = tile_m;
-        ml = nl;
+        s2 = pair(o.x * f, o.y * f);
+        m = ref = tile_m;
       }
-      const uint64_t nml = pair(-ml, -ml);
+      const uint64_t nref = pair(-ref, -ref);
 #pragma unroll
       for (int i = 0; i < kU * 4; i += 3 - WN) {
         const float a = Word<T>::get(wd[i], 0);
         const float b = WN == 2 ? Word<T>::get(wd[i], 1) : Word<T>::get(wd[i + 1], 0);
-        const float2 e = unpair(fma2(pair(a, b), l2e, nml));
+        const float2 e = unpair(mul2(add2(pair(a, b), nref), l2e));
         s2 = add2(s2, pair(ex2(e.x), ex2(e.y)));
       }
 #pragma unroll
@@ -411,8 +412,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
     float s = sp.x + sp.y;               // NaN: a NaN, or an infinity, among the logits
     float wm = m;
     for (int o = 16; o; o >>= 1) wm = fmaxf(wm, __shfl_xor_sync(0xffffffffu, wm, o));
-    // 2^((m - wm) log2(e)), and ml's rounding taken out
-    float ws = m == kNegInf ? s : s * ex2((m - wm) * kLog2e - fmaf(m, kLog2e, -ml));
+    float ws = m == kNegInf ? s : s * ex2((m - wm) * kLog2e);
     for (int o = 16; o; o >>= 1) ws += __shfl_xor_sync(0xffffffffu, ws, o);
     const float m2 = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));   // of two threads
     if (!(lane & 1)) maxima[threadIdx.x >> 1] = m2;
@@ -564,11 +564,12 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
       const float mt = __uint_as_float((uint32_t)(u >> 32)), st = __uint_as_float((uint32_t)u);
       sum += mt == kNegInf ? st : (double)(st * ex2((mt - M) * kLog2e));
     }
-    const double lse = (double)M + log(sum);
+    const double lg = log(sum);
     const bool fin = p.finished && p.finished[gk];
     row_b[k] = (double)b;
-    row_lse[k] = lse;
-    row_kind[k] = !isfinite(b) ? 1 : fin ? 2 : isfinite(lse) ? 0 : 1;
+    row_log[k] = lg;
+    row_max[k] = M;
+    row_kind[k] = !isfinite(b) ? 1 : fin ? 2 : isfinite(M) && isfinite(lg) ? 0 : 1;
   }
   if (threadIdx.x == 0) survivors = 0;
   __syncthreads();
@@ -584,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
     if (kind == 0) {
       const unsigned long long key = all[i];
       if (key != 0ull) {
-        sc = row_b[k] + ((double)key_value(key) - row_lse[k]);
+        sc = row_b[k] + (((double)key_value(key) - (double)row_max[k]) - row_log[k]);
         c.score = score_bits(sc);
         c.tie = make_tie(k, (uint32_t)(key >> 32), key_index(key));
       }

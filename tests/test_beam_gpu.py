@@ -122,6 +122,54 @@ def test_select_lowest_values_as_mask():
     check_select(x, s, 24)
 
 
+def log_softmax_select(logits, beam_scores, n):
+    """As ``plain_select``, with the log-softmax formed from differences to the maximum, which
+    64 bits hold even where the logits are too large for sums with them."""
+    G, K = beam_scores.shape
+    x = logits.double().reshape(G, K, -1).cpu()
+    V = x.shape[-1]
+    sc = beam_scores.double().cpu()[..., None] + torch.log_softmax(x, -1)
+    v, i = torch.sort(sc.reshape(G, K * V), dim=-1, descending=True, stable=True)
+    return v[:, :n], (i // V)[:, :n].int(), (i % V)[:, :n]
+
+
+def check_large(x, s, n):
+    got = beam_select(x, s, num_out=n)
+    rs, rb, rt = log_softmax_select(x, s, n)
+    assert torch.equal(got[1].cpu(), rb) and torch.equal(got[2].cpu(), rt)
+    err = (got[0].cpu().double() - rs).abs()
+    assert (err <= rs.abs() * 2.0 ** -24 + 2.0 ** -20).all()      # as in check_select
+
+
+MASKS = [(dt, m) for dt in (torch.float32, torch.bfloat16, torch.float16)
+         for m in ("min", -5e9, -1e10, -1e20, -1e30, -1e37) if m == "min" or dt != torch.float16]
+
+
+@pytest.mark.parametrize("dtype,mask", MASKS)
+def test_select_large_negative_masks(dtype, mask):
+    """Finite masks of any size, over most of a row, over whole tiles, threads and splits of
+    it and over all of it."""
+    mask = torch.finfo(dtype).min if mask == "min" else mask
+    x, s = rand(3, 4, 20011, dtype, 31)
+    gone = torch.rand(4, 20011, device=DEV, generator=torch.Generator(device=DEV).manual_seed(32))
+    x[:4].masked_fill_(gone < 0.99, mask)
+    x[4, :15000] = mask                  # the first tiles of most threads
+    x[5, 5000:] = mask
+    x[6] = mask                          # all of a row: uniform
+    x[7, :20010] = mask                  # one token left
+    x[8:, 3:20000] = mask
+    for n in (1, 8, 64):
+        check_large(x, s, n)
+
+
+@pytest.mark.parametrize("dtype,size", [(torch.float32, 1e38), (torch.bfloat16, 1e38),
+                                        (torch.float32, 1e9), (torch.float16, 2e4)])
+def test_select_logits_of_any_size(dtype, size):
+    x, s = rand(2, 4, 5001, torch.float32, 33, scale=1.0)
+    x = (x.clamp(-3.2, 3.2) * size).to(dtype)
+    check_large(x, s, 8)
+
+
 def test_select_finished_beams():
     x, s = rand(6, 4, 1000, torch.bfloat16, 5)
     fin = torch.zeros(6, 4, dtype=torch.bool, device=DEV)
