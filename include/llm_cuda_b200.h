@@ -293,7 +293,9 @@ LLMC_API int llmc_shared_prefix_decode(
  * Beam selection: for each of G prompts the n best continuations of its K beams,
  *   score[k, v] = beam_scores[k] + logits[k, v] - logsumexp(logits[k, :]),
  * in descending order, ties to the lowest k * V + v (inside a beam the order is that of
- * the logits).  No counterpart in the reference, which picks greedily
+ * the logits; beams of equal logits and scores tie wherever their rows begin).  A log-sum-exp
+ * is good to 2^-20: candidates of different beams that are closer come in either order.
+ * No counterpart in the reference, which picks greedily
  * (src/llm_cuda/models/llama3/model.py:214); stands beside llmc_argmax.
  *   logits: row g * K + k at logits + (g * K + k) * row_stride elements.
  *   beam_scores [G, K] fp32; finished [G, K] bytes or NULL: a finished beam offers the

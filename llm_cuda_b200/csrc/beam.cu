@@ -199,6 +199,35 @@ struct Word<__nv_bfloat16> {
   static __device__ __forceinline__ float top(uint32_t a) { return fmaxf(get(a, 0), get(a, 1)); }
 };
 
+// Vectors of a row by index from the aligned ones that were fetched: vector v holds elements
+// [v VEC, v VEC + VEC) of the row, the fetched ones begin h elements (0 < h < VEC) earlier.  The
+// rest of a lane's vectors is in the next lane, the last lane's in the first lane's next one.
+// Vectors from `left` on are -inf.
+template <typename T>
+__device__ __forceinline__ void realign(uint4 (&tile)[kU], const uint4& behind, int h, int lane,
+                                        int left) {
+  const int bytes = h * (int)sizeof(T);
+#pragma unroll
+  for (int u = 0; u < kU; ++u) {
+    const uint4 a = tile[u], b = u + 1 < kU ? tile[u + 1 < kU ? u + 1 : u] : behind;
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[4 + i] = __shfl_sync(0xffffffffu, lane ? w[i] : w[4 + i], (lane + 1) & 31);
+    if (bytes & 8)
+#pragma unroll
+      for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    if (bytes & 4)
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    if (bytes & 2)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __byte_perm(w[i], w[i + 1], 0x5432);
+    constexpr uint32_t F = Word<T>::kNegInf;
+    tile[u] = u * 32 + lane < left ? make_uint4(w[0], w[1], w[2], w[3]) : make_uint4(F, F, F, F);
+  }
+}
+
 // How many of the n descending entries of a are better than `key`.
 __device__ __forceinline__ int count_better(const unsigned long long* a, int n,
                                             unsigned long long key) {
@@ -325,16 +354,20 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
       continue;
     }
     const T* x = reinterpret_cast<const T*>(p.logits) + ((long long)g * K + row) * p.row_stride;
-    // Vectors are 16-byte aligned: vector v holds elements [v * VEC - h, v * VEC - h + VEC).
+    // A row is cut by the index of its elements, wherever it begins: vector v holds elements
+    // [v VEC, v VEC + VEC).  Rows of equal logits so have the same sums, bit for bit, and tie.
+    // A row that begins h elements behind a 16-byte boundary is fetched from that boundary on
+    // and its vectors are put together from two neighbours (see realign; 64 prompts of 8 beams,
+    // V 128255: 48.7 us, cut by address, which ties of rows at odd strides do not survive, 41.7).
     const int h = (int)((reinterpret_cast<uintptr_t>(x) / sizeof(T)) % VEC);
-    const int nvec = (V + h + VEC - 1) / VEC;
+    const int nvec = (V + VEC - 1) / VEC;
     const int v0 = (int)((long long)nvec * split / S), v1 = (int)((long long)nvec * (split + 1) / S);
     // A warp's vectors are contiguous, so its later elements have larger indices.
     const int w0 = v0 + (int)((long long)(v1 - v0) * warp / kWarps);
     const int w1 = v0 + (int)((long long)(v1 - v0) * (warp + 1) / kWarps);
-    // Tiles of whole vectors of this warp's part: [whole0, whole1).
+    // Fetched vectors that are whole: [whole0, whole1).
     const uint4* vec = reinterpret_cast<const uint4*>(x - h) + lane;
-    const int whole0 = h ? 1 : 0, whole1 = min(w1, (V + h) / VEC);
+    const int last = h ? w1 + 1 : w1, whole0 = h ? 1 : 0, whole1 = min(last, (V + h) / VEC);
     auto load = [&](int base, uint4 (&raw)[kU]) {
       if (base >= whole0 && base + 32 * kU <= whole1) {
 #pragma unroll
@@ -348,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
         const long long e0 = (long long)v * VEC - h;
         constexpr uint32_t F = Word<T>::kNegInf;
         raw[u] = make_uint4(F, F, F, F);
-        if (v >= w1) continue;
+        if (v >= last) continue;
         if (v >= whole0 && v < whole1) {
           raw[u] = __ldg(vec + base + u * 32);
         } else {
@@ -373,6 +406,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
     for (int base = w0; base < w1; base += 32 * kU) {
       uint4 next[kU];
       load(base + 64 * kU, next);
+      if (h) realign<T>(cur, ahead[0], h, lane, w1 - base);
       const uint32_t* wd = reinterpret_cast<const uint32_t*>(cur);
       uint32_t mw = wd[0];
 #pragma unroll
@@ -463,9 +497,9 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
         const int tw1 = v0 + (int)((long long)(v1 - v0) * (tw + 1) / kWarps);
         for (int b = 0; b < per_cell; ++b) {
           const int u = lane / VEC, v = tw0 + (c * per_cell + b) * 32 * kU + u * 32 + (th & 31);
-          const long long idx = (long long)v * VEC - h + lane % VEC;
+          const long long idx = (long long)v * VEC + lane % VEC;
           float f = kNegInf;
-          const bool in = lane < kU * VEC && v < tw1 && idx >= 0 && idx < V;
+          const bool in = lane < kU * VEC && v < tw1 && idx < V;
           if (in) f = to_f32(x[idx]);
           const bool pass = in && f >= bound;
           const unsigned vote = __ballot_sync(0xffffffffu, pass);
@@ -504,7 +538,17 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
       const int end = min(w1, w0 + (c + 1) * per_cell * 32 * kU);
       for (int base = w0 + c * per_cell * 32 * kU; base < end; base += 32 * kU) {
         uint4 raw[kU];
-        load(base, raw);
+        if (h == 0) {
+          load(base, raw);
+        } else {
+          T* r = reinterpret_cast<T*>(raw);
+#pragma unroll
+          for (int i = 0; i < kU * VEC; ++i) {
+            const long long idx = (long long)(base + i / VEC * 32 + lane) * VEC + i % VEC;
+            constexpr uint32_t F = Word<T>::kNegInf;
+            r[i] = idx < V ? x[idx] : *reinterpret_cast<const T*>(&F);
+          }
+        }
         const uint32_t* wd = reinterpret_cast<const uint32_t*>(raw);
         const bool strict = top.full && top.tau >= bound;
         const float lo = top.full ? fmaxf(top.tau, bound) : bound;
@@ -520,8 +564,8 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
           const int bit = pass ? __ffs(mask) - 1 : 0;
           mask &= mask - 1;
           const int v = base + (bit / VEC) * 32 + lane;
-          const long long idx = (long long)v * VEC - h + bit % VEC;
-          pass = pass && v < w1 && idx >= 0 && idx < V;
+          const long long idx = (long long)v * VEC + bit % VEC;
+          pass = pass && v < w1 && idx < V;
           const float f = pass ? to_f32(x[idx]) : 0.f;
           unsigned vote = __ballot_sync(0xffffffffu, pass);
           if (top.count + __popc(vote) > kCap) {

@@ -33,7 +33,9 @@ def beam_select(
     ``[G, K]``: a finished beam offers ``eos_token_id`` at its own score and nothing else.
     A beam with a score or log-sum-exp that is not finite offers its tokens at ``-inf``.
     Returns ``(scores fp32, beams int32, tokens int64)``, each ``[G, num_out]``, best first,
-    ties to the lowest (beam, token).
+    ties to the lowest (beam, token); beams of equal logits and scores tie wherever their rows
+    begin.  A log-sum-exp is good to 2^-20: candidates of different beams that are closer come
+    in either order.
     """
     lib = N.load()
     if not logits.is_cuda or not beam_scores.is_cuda:

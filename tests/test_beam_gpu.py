@@ -170,6 +170,34 @@ def test_select_logits_of_any_size(dtype, size):
     check_large(x, s, 8)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V,pad", [(50257, 0), (4099, 0), (1001, 2), (20000, 3), (128255, 0)])
+def test_select_equal_rows_tie_at_any_alignment(V, pad, dtype):
+    """Rows of equal logits have equal scores wherever they begin: the lowest beam comes first."""
+    for seed, K, n in ((1, 8, 64), (2, 5, 10), (3, 16, 33), (4, 32, 64)):
+        x, s = rand(2, 1, V, dtype, 40 + seed)
+        wide = torch.zeros(2 * K, V + pad, dtype=dtype, device=DEV)
+        wide[:, :V] = x.repeat_interleave(K, 0)
+        check_select(wide[:, :V], s.expand(2, K).contiguous(), n)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_select_rows_at_every_offset(dtype):
+    """Rows that begin anywhere between two 16-byte boundaries, of lengths around the vectors
+    and tiles, with few distinct values (ties, cells and lists of many equal logits) and many;
+    what lies around a row is NaN."""
+    per = 16 // torch.empty(0, dtype=dtype).element_size()
+    for V in (1, 2, per - 1, per, per + 1, 3 * per + 1, 1024, 1025, 8191, 8192 + per - 1, 40003):
+        for off in range(per):
+            few = (off + V) % 3 == 0
+            x, s = rand(1, 3, V, dtype, V + off, scale=0.01 if few else 3.0)
+            if few:
+                x = (x * 400).round() / 4
+            wide = torch.full((3, V + per + 1), float("nan"), dtype=dtype, device=DEV)
+            wide[:, off:off + V] = x
+            check_select(wide[:, off:off + V], s, min(64, 3 * V))
+
+
 def test_select_finished_beams():
     x, s = rand(6, 4, 1000, torch.bfloat16, 5)
     fin = torch.zeros(6, 4, dtype=torch.bool, device=DEV)
