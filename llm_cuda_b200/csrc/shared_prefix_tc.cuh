@@ -29,9 +29,14 @@
 // (measured with narrow tiles against: 4 groups of 256 rows x 8192 tokens 78 us and 72, 256
 // rows x 512 tokens 24.9 and 23.2).
 //
-// The running maximum is only raised when it would grow by more than 8 (log2): weights up
-// to 2^8 are harmless in 16 bits, and O is then rarely rescaled.  Rounded to 16 bits: the
-// weights P, as a tensor-core operand; the maximum, the sum, S and O are fp32.
+// The running maximum is only raised when it would grow by more than 8 (log2, fp16: 4): weights
+// above 1 are harmless in 16 bits, and O is then rarely rescaled.  Rounded to 16 bits: the
+// weights P, as a tensor-core operand (a relative 2^-9 or 2^-12 each, at random: the plain
+// 64-bit result is off by up to 40% more than with fp32 weights; the weights of paged_decode are
+// rounded alike, and two products of halves would double the tensor cores' work); the maximum,
+// the sum, S and O are fp32.  fp16 has few exponents: its weights are 2^8 times as large (2^12
+// at most, finite up to scores of 2^26), so that one of 2^-22 of the greatest still has all its
+// bits and the smaller ones are off by 2^-33 of the greatest at most.
 //
 // Bound: HBM where few rows share a token (8 sequences of 131 thousand: 105 us for 541 MB, 79%
 // of a plain copy's rate with start-up and join); with 128 sequences the chain of product,
@@ -48,6 +53,11 @@ namespace tc {
 constexpr int kChunk = 128;        // tokens of a chunk (MMA N of S, K of P V)
 constexpr int kRing = 8;            // segments the producer may be ahead
 constexpr int kThreads = 384;      // two softmax warpgroups, one for the producer and the issuer
+// Of the weights, log2: how far the maximum may lag behind, and their scale.
+template <typename T>
+constexpr float kLag = __is_same(T, __half) ? 4.f : 8.f;
+template <typename T>
+constexpr float kScale = __is_same(T, __half) ? 8.f : 0.f;
 
 struct TcParams {
   Params p;
@@ -917,6 +927,8 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
     const float kNegInf = __int_as_float(0xff800000);
     const float sc = p.scale_log2;                     // positive
     const uint64_t sc2 = pair(sc, sc);
+    // the scaled score whose weight is 1
+    auto zero_of = [&](float m) { return m == kNegInf ? 0.f : fmaf(m, sc, -kScale<T>); };
     const int narrow = tp.nb * p.R;
     const int box = min(p.P, kChunk), bsh = 31 - __clz(box);
     int k = 0, it = 0, n_items = 0, n_o = 0;
@@ -988,8 +1000,8 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
             landed(v1[1]);
             mx = fmaxf(mx, block_max(v1));
           }
-          // Raise the reference maximum where the weights would pass 2^8.
-          const bool raise = start || (mx - m) * sc > 8.f;
+          // Raise the reference maximum where the weights would grow too large.
+          const bool raise = start || (mx - m) * sc > kLag<T>;
           if (__any_sync(0xffffffffu, raise)) {
             const float f = !raise ? 1.f : m == kNegInf ? 0.f : ex2((m - mx) * sc);
             m = raise ? mx : m;
@@ -1009,7 +1021,7 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
               }
             }
           }
-          const float ms = m == kNegInf ? 0.f : m * sc;
+          const float ms = zero_of(m);
           const uint64_t nm2 = pair(-ms, -ms);
           auto weigh = [&](const uint32_t (&v)[2][32]) {
 #pragma unroll
@@ -1090,7 +1102,7 @@ parts_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ 
                     __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
             }
           }
-          if (write) pl[r] = l == 0.f ? kNegInf : (m == kNegInf ? 0.f : m * sc) + log2f(l);
+          if (write) pl[r] = l == 0.f ? kNegInf : zero_of(m) + log2f(l);
         }
         fence_before();   // O is read: the next segment's products may overwrite it
       } else if (write) {

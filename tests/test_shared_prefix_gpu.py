@@ -396,3 +396,47 @@ def test_every_page_size_of_the_tensor_cores(P, d, dtype):
               [301, 463, 700, 9, 330] + [133 + (5 * i) % 37 for i in range(70)], 8, 4, d, P, dtype,
               seed=P + d)
     b.check(b.run())
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("own", [False, True])
+@pytest.mark.parametrize("log2_weight", [-12.0, -20.5, -25.5, -28.0])
+def test_small_weights_beside_a_large_one_fp16(log2_weight, own, d):
+    """One token with (nearly) all of the weight and a value of 0, the others with so little that
+    fp16 would drop them, and values of 1000.  Weights are 2^8 times their size against the
+    greatest; where that is a subnormal of fp16 it is rounded by 2^-25, which is 2^-33 of the
+    normaliser: n 2^-33 1000 beside the usual bound."""
+    n = 250
+    lens = [n + 1] * 3
+    b = Batch([3], [0 if own else n], lens, 4, 2, d, 16, HF, seed=21)
+    b.q.fill_(1.0)
+    top = -log2_weight * math.log(2.0) * d ** 0.5 / d       # score 0 for the others
+    for i in range(3):
+        b.k[i].zero_()
+        b.v[i].fill_(1000.0)
+        b.k[i][:, 17] = top
+        b.v[i][:, 17] = 0.0
+        for t in range(n + 1):
+            page = int(b.bt[i, t // 16])
+            b.kp[page, :, t % 16] = b.k[i][:, t].to(DEV)
+            b.vp[page, :, t % 16] = b.v[i][:, t].to(DEV)
+    out = b.run()
+    q = b.q[0, :2].double().cpu()
+    p = torch.softmax(torch.einsum("hd,htd->ht", q, b.k[0].double()) * d ** -0.5, -1)
+    o = torch.einsum("ht,htd->hd", p, b.v[0].double())
+    # the usual bound (above), A = o here; fp16 results below 2^-14 are rounded by 2^-25
+    e = (d + 4) * 2.0 ** -24 * float(b.k[0][0, 17].abs().sum()) * d ** -0.5
+    rel = 2 * 2.0 ** -11 + 2 * e + 2 * 2.0 ** -21 + (2 * n + 18) * 2.0 ** -24
+    tol = rel * o + n * 2.0 ** -33 * 1000 + 2.0 ** -25
+    got = out.double().cpu().view(3, 2, 2, d)
+    assert ((got - o[None, :, None]).abs() <= tol[None, :, None]).all(), \
+        float(((got - o[None, :, None]).abs() / tol[None, :, None]).max())
+    assert int(b.status.item()) == 0
+
+
+@pytest.mark.parametrize("size", [30.0, 1000.0])
+def test_large_scores_fp16(size):
+    """Scores that differ by thousands: each row is (nearly) one value, and finite."""
+    b = Batch([4], [700], [701, 740, 950, 1160], 8, 2, 128, 16, HF, seed=17)
+    b.q *= size
+    b.check(b.run())
