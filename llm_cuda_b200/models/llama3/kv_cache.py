@@ -226,9 +226,10 @@ class PagedKVLayerCache:
         if seq != 1:
             raise ValueError("rope_append_decode takes one new token per sequence")
         if self.shared is not None:
+            self._check_shared_step(q, out, partition_tokens)   # a refused call appends nothing
             q_rot = self.append_rotary(q, k, v, rope,
                                        q_out=q_out if q_out is None else q_out.view(q.shape))
-            return self.decode(q_rot, out=out, partition_tokens=partition_tokens)
+            return self.decode(q_rot, out=out)
         res = rope_append_decode(q, k, v, self.key_pages, self.value_pages, self.block_table,
                                  self.seq_lens, rope.cos, rope.sin, host_lens=self.host_lengths,
                                  partition_tokens=partition_tokens, out=out, q_out=q_out,
@@ -236,6 +237,20 @@ class PagedKVLayerCache:
                                  early_tables=early_tables)
         self.host_lengths = [x + 1 for x in self.host_lengths]
         return res
+
+    def _check_shared_step(self, q: torch.Tensor, out: torch.Tensor | None,
+                           partition_tokens: int | None) -> None:
+        if partition_tokens:
+            raise ValueError("decode over shared prefixes takes no partition_tokens")
+        if q.dim() != 4 or q.shape[0] != self.batch_size or q.shape[1] % self.num_kv_heads or \
+                q.shape[2] != 1 or q.shape[3] != self.head_dim or q.dtype != self.dtype or \
+                q.device != self.key_pages.device:
+            raise ValueError("q must be [batch, heads, 1, head_dim] in the cache's dtype, on its "
+                             "device, with a multiple of its heads")
+        if out is not None and (out.shape not in (q.shape, q[:, :, 0].shape)
+                                or out.dtype != q.dtype or out.device != q.device
+                                or not out.is_contiguous()):
+            raise ValueError("out must be contiguous and match q")
 
     def advance_host_lengths(self, n: int) -> None:
         """Mirror ``n`` appends replayed from a CUDA graph (the device already advanced)."""

@@ -147,3 +147,19 @@ def test_beam_select_refuses_a_vocabulary_past_its_ties():
     lib = N.load()
     assert _select(lib, V=(1 << 27) + 1, stride=1 << 28) == -2
     assert b"2^27" in lib.llmc_last_error_string()
+
+
+def test_refused_step_over_shared_prefixes_appends_nothing():
+    from llm_cuda_b200.models.llama3 import BeamKVCache
+
+    c = BeamKVCache(1, 2, 64, 40, 16, "cpu", torch.bfloat16, [20], beams=2)
+    lc = c.get_layer(0)
+    lc.host_lengths = [20, 20]
+    q, k = torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16), torch.zeros(2, 2, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="partition_tokens"):
+        lc.rope_append_decode(q, k, k, None, partition_tokens=64)
+    with pytest.raises(ValueError, match="out must"):
+        lc.rope_append_decode(q, k, k, None, out=torch.zeros(2, 4, 1, 32, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="q must"):
+        lc.rope_append_decode(q[:, :3], k, k, None)
+    assert lc.host_lengths == [20, 20] and lc.seq_lens.tolist() == [0, 0]

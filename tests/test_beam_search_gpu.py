@@ -207,3 +207,21 @@ def test_beam_step_in_a_graph():
         torch.cuda.synchronize()
         assert torch.equal(sc, want[0]) and torch.equal(tok, want[1])
     cache.check_status()
+
+
+def test_refused_step_leaves_the_cache_as_it_was():
+    m = tiny(torch.bfloat16, seed=8)
+    ids = torch.randint(0, 512, (1, 21), generator=torch.Generator().manual_seed(4)).to(DEV)
+    cache = m.make_beam_cache([21], 2, 40)
+    tok = m.prefill(ids, cache.leaders()).topk(2).indices.view(-1)
+    cache.fork()
+    before = cache.pools.clone()
+    with pytest.raises(ValueError, match="partition_tokens"):
+        m.decode_step(tok, cache, partition_tokens=256)
+    lc = cache.get_layer(0)
+    q = torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="out must"):
+        lc.rope_append_decode(q, q[:, :2], q[:, :2], m.rope, out=q[..., :32])
+    for lc in cache.layer_caches:
+        assert lc.seq_lens.tolist() == [21, 21] and lc.host_lengths == [21, 21]
+    assert torch.equal(cache.pools.nan_to_num(), before.nan_to_num())
