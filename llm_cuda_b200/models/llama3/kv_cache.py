@@ -425,7 +425,8 @@ class GraphedDecodeStep:
     graph launch per step instead of several Python-issued launches: the host cost of
     a step is that of ``cudaGraphLaunch``.  By default the step uses the balanced
     split, which the kernel recomputes from the device lengths at every replay, so
-    the work stays even across SMs as the contexts grow.
+    the work stays even across SMs as the contexts grow.  A cache with shared prefixes
+    takes its own step (RoPE and append, then ``shared_prefix_decode``).
     """
 
     def __init__(self, cache: PagedKVLayerCache, rope: RopeTable, q: torch.Tensor,
@@ -435,6 +436,8 @@ class GraphedDecodeStep:
 
         self.cache, self.rope, self.q, self.k, self.v = cache, rope, q, k, v
         B, Hq, d = q.shape[0], q.shape[1], q.shape[-1]
+        if cache.shared is not None:
+            cache._check_shared_step(q, out, partition_tokens)
         self.partition_tokens = BALANCED if partition_tokens is None else partition_tokens
         self.out = out if out is not None else torch.empty(B, Hq, d, dtype=q.dtype,
                                                            device=q.device)
@@ -457,6 +460,12 @@ class GraphedDecodeStep:
 
     def _step(self):
         c = self.cache
+        if c.shared is not None:
+            rope_append(self.q, self.k, self.v, c.key_pages, c.value_pages, c.block_table,
+                        c.seq_lens, c.status, cos=self.rope.cos, sin=self.rope.sin,
+                        q_out=self.q_rot.view(self.q.shape))
+            c.decode(self.q_rot, out=self.out)
+            return
         rope_append_decode(self.q, self.k, self.v, c.key_pages, c.value_pages, c.block_table,
                            c.seq_lens, self.rope.cos, self.rope.sin,
                            partition_tokens=self.partition_tokens, out=self.out,

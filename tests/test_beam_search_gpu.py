@@ -225,3 +225,34 @@ def test_refused_step_leaves_the_cache_as_it_was():
     for lc in cache.layer_caches:
         assert lc.seq_lens.tolist() == [21, 21] and lc.host_lengths == [21, 21]
     assert torch.equal(cache.pools.nan_to_num(), before.nan_to_num())
+
+
+def test_graphed_step_over_shared_prefixes():
+    """A captured step of a beam layer: the results of eager steps, bit for bit (the kernel that
+    reads the prompt once per prompt rounds otherwise than the one that reads it per beam)."""
+    from llm_cuda_b200.models.llama3.kv_cache import GraphedDecodeStep
+
+    def make():
+        c = BeamKVCache(1, 2, 64, 400, 16, DEV, torch.bfloat16, [300, 130], 3,
+                        generator=torch.Generator().manual_seed(5))
+        c.pools.copy_(torch.randn(c.pools.shape, generator=torch.Generator().manual_seed(6)))
+        c.fork()
+        return c
+
+    g = torch.Generator().manual_seed(7)
+    rope = RopeTable(400, 64, 500000.0, DEV, torch.bfloat16)
+    eager, graphed = make(), make()
+    q, k, v = (torch.zeros(6, h, 1, 64, dtype=torch.bfloat16, device=DEV) for h in (8, 2, 2))
+    with pytest.raises(ValueError, match="partition_tokens"):
+        GraphedDecodeStep(graphed.get_layer(0), rope, q, k, v, partition_tokens=128)
+    step = GraphedDecodeStep(graphed.get_layer(0), rope, q, k, v)
+    for _ in range(4):
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, generator=g))
+        want = eager.get_layer(0).rope_append_decode(q, k, v, rope)
+        got = step.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want[:, :, 0])
+    assert graphed.get_layer(0).host_lengths == eager.get_layer(0).host_lengths == [304] * 3 + [134] * 3
+    assert torch.equal(graphed.pools, eager.pools)
+    graphed.check_status()
