@@ -459,11 +459,11 @@ int llmc_beam_select(const void* logits, long long row_stride, const float* beam
   if (row_stride < V) return fail(LLMC_EINVAL, "llmc_beam_select: row_stride smaller than V");
   if (finished && (eos < 0 || eos >= V))
     return fail(LLMC_EINVAL, "llmc_beam_select: finished beams need 0 <= eos < V");
+  if (G == 0) return LLMC_OK;   // an empty tensor may have no address
   if (!logits || !beam_scores || !out_scores || !out_beams || !out_tokens)
     return fail(LLMC_EINVAL, "llmc_beam_select: NULL pointer argument");
   if (reinterpret_cast<uintptr_t>(logits) & (dtype == LLMC_F32 ? 3 : 1))
     return fail(LLMC_EINVAL, "llmc_beam_select: misaligned logits");
-  if (G == 0) return LLMC_OK;
   cudaError_t e = llmc::launch_beam_select(logits, row_stride, beam_scores, finished, out_scores,
                                            out_beams, out_tokens, G, K, V, n, eos, dtype,
                                            (cudaStream_t)stream);

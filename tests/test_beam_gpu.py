@@ -340,3 +340,12 @@ def test_reorder_leaves_a_bad_prompt_alone():
         assert torch.equal(pools, before[0]) and torch.equal(bt[4:8], before[1][4:8])
         with pytest.raises(N.DeviceStatusError, match=word):
             N.raise_on_status(st)
+
+
+def test_no_prompts():
+    s, b, t = beam_select(torch.zeros(0, 100, device=DEV), torch.zeros(0, 4, device=DEV), num_out=8)
+    assert s.shape == b.shape == t.shape == (0, 8)
+    s, b, t = beam_select(torch.zeros(0, 4, 100, device=DEV, dtype=torch.bfloat16),
+                          torch.zeros(0, 4, device=DEV),
+                          finished=torch.zeros(0, 4, dtype=torch.bool, device=DEV), eos_token_id=1)
+    assert s.shape == b.shape == t.shape == (0, 4)

@@ -163,3 +163,10 @@ def test_refused_step_over_shared_prefixes_appends_nothing():
     with pytest.raises(ValueError, match="q must"):
         lc.rope_append_decode(q[:, :3], k, k, None)
     assert lc.host_lengths == [20, 20] and lc.seq_lens.tolist() == [0, 0]
+
+
+def test_no_prompts_need_no_pointers():
+    """An empty tensor's address is NULL."""
+    lib = N.load()
+    assert lib.llmc_beam_select(None, 100, None, None, None, None, None, 0, 4, 100, 4, -1,
+                                N.LLMC_BF16, None) == 0
