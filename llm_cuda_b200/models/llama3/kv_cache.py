@@ -162,6 +162,11 @@ class PagedKVLayerCache:
         elif any(t.shape != (num_pages, num_kv_heads, page_size, head_dim) or t.dtype != dtype
                  or not t.is_contiguous() for t in (key_pages, value_pages)):
             raise ValueError("pools must be contiguous [num_pages, Hkv, page_size, d] in dtype")
+        given = [key_pages, value_pages]
+        if shared is not None:
+            given += [shared.group_starts, shared.shared_lens]
+        if any(t.device != self.block_table.device for t in given):
+            raise ValueError("pools and shared prefixes must be on the cache's device")
         self.key_pages = key_pages
         self.value_pages = value_pages
         self.shared = shared

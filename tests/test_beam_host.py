@@ -170,3 +170,20 @@ def test_no_prompts_need_no_pointers():
     lib = N.load()
     assert lib.llmc_beam_select(None, 100, None, None, None, None, None, 0, 4, 100, 4, -1,
                                 N.LLMC_BF16, None) == 0
+
+
+def test_cache_refuses_pools_and_groups_of_another_device():
+    """A kernel would be given their addresses."""
+    from llm_cuda_b200.models.llama3 import PagedKVLayerCache, SharedPrefix
+
+    kv = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    far = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16, device="meta")
+    ok = PagedKVLayerCache(2, 64, 64, 16, "cpu", torch.bfloat16, key_pages=kv, value_pages=kv.clone(),
+                           shared=SharedPrefix([0, 1], [5], "cpu"))
+    assert ok.key_pages is kv
+    for k, v in ((far, far), (kv, far), (far, kv)):
+        with pytest.raises(ValueError, match="device"):
+            PagedKVLayerCache(2, 64, 64, 16, "cpu", torch.bfloat16, key_pages=k, value_pages=v)
+    with pytest.raises(ValueError, match="device"):
+        PagedKVLayerCache(2, 64, 64, 16, "cpu", torch.bfloat16, key_pages=kv, value_pages=kv,
+                          shared=SharedPrefix([0, 1], [5], "meta"))
