@@ -14,12 +14,15 @@
 // CTA fetches the tasks' lists and sums through distributed shared memory and ranks the
 // candidates by their scores in the same way.
 // Bound: the logits are read once from HBM; then the exponentials (16 a cycle and SM).
-// Measured on 64 prompts of 8 beams, 131 MB of bf16 logits: 41 us (floor 20 us), some 29 of
-// them the stream; with lists kept up to date while streaming instead of cells 104 us.
+// Measured on 64 prompts of 8 beams, 131 MB of bf16 logits: 41 us captured and called (floor 20
+// us), some 29 of them the stream; with lists kept up to date while streaming instead of cells
+// 104 us.  A CTA's tasks run one after another: nothing streams while a row is ranked (8 prompts
+// of 32 beams, two rows a CTA: 72 us, floor 10).
 //
 // Sums of exponentials are held in fp32 per thread, joined in fp32 inside a split and in
-// fp64 across splits; scores are ranked in fp64 (candidates of different beams are often
-// closer than fp32 tells apart) and rounded once to fp32.
+// fp64 across splits: a log-sum-exp is good to 2^-20.  Scores are ranked in
+// fp64 (at -12 and less, candidates of different beams are often closer than fp32 tells apart)
+// and rounded once to fp32.
 //
 // beam_reorder: beam i of a prompt continues from beam parent[i].  See below.
 #include <climits>
@@ -719,8 +722,9 @@ __global__ void __launch_bounds__(kThreads, 2) beam_select_kernel(const SelectPa
 //
 // The copies of a prompt form a permutation with repeats, in place: a thread loads one
 // 16-byte vector of all K pages, then stores them, so no copy sees another's result.  The
-// table is moved the same way, a thread per column.  Bound: HBM (the moved tokens; 112.5 us
-// for 638 MB, 87% of a plain copy's rate), and at small sizes the launch (2.9 us).
+// table is moved the same way, a thread per column.  Bound: HBM (the moved tokens; 113 us for
+// 638 MB, 86% of a plain copy's rate), and at small sizes the launch (2.9 us captured, 9.3 us
+// from the host).
 struct ReorderParams {
   uint8_t* pools;              // [layers][2][num_pages][Hkv][P][d]
   const int32_t* own_table;    // [G * K, max_pages]

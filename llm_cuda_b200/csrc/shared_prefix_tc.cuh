@@ -40,8 +40,9 @@
 //
 // Bound: HBM where few rows share a token (8 sequences of 131 thousand: 105 us for 541 MB, 79%
 // of a plain copy's rate with start-up and join); with 128 sequences the chain of product,
-// softmax and product (119 us, of which the tensor cores need 42), some 2,100 cycles per item
-// of 128 x 128.  Before the first scores some 12 us pass, on code and tables from HBM.
+// softmax and product (120 us, of which the tensor cores need 42), some 2,100 cycles per item
+// of 128 x 128.  (Device times of captured calls; a call from the host takes 115 and 130 us.)
+// Before the first scores some 12 us pass, on code and tables from HBM.
 #pragma once
 
 #include "shared_prefix.cuh"

@@ -50,8 +50,9 @@ def shared_prefix_decode(
     ``group_starts[g] .. group_starts[g + 1] - 1``.  ``shared_lens`` int32 ``[G]``: how many
     first tokens the group's sequences have in common (any number, 0 for none).  Every row
     of ``block_table`` names all pages of its sequence.  ``max_group`` bounds the sequences
-    of a group (default: the batch); it sizes the workspace, and sequences of a group
-    beyond it are decoded by themselves.  Sequences of length 0 give zeros.  All lengths
+    of a group (default: the batch); it sizes the workspace (512 sequences of 64/8 heads in as
+    many groups: 104 MB with 1, 630 MB with the default), and sequences of a group beyond it
+    are decoded by themselves.  Sequences of length 0 give zeros.  All lengths
     are read on the device, so the call can be captured in a CUDA graph.
     """
     lib = N.load()
